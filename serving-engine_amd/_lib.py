@@ -1,4 +1,5 @@
-"""ctypes binding of libkvhot.so, the C-ABI library declared in include/kvhot.h.
+"""ctypes binding of libkvhot.so, the C-ABI library declared in include/kvhot.h
+and include/kvhot_layer.h.
 
 torch is imported before the library is opened so that libkvhot binds to the
 HIP runtime torch already loaded (both carry SONAME libamdhip64.so.7): device
@@ -84,6 +85,36 @@ SIGNATURES = {
     ),
 }
 
+# The same for include/kvhot_layer.h.
+LAYER_SIGNATURES = {
+    "kvhot_build_block_tables": (
+        _int,
+        [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "kvhot_norm_rope": (
+        _int,
+        [_vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _i64p, _vp, _vp, _int, ctypes.c_float, _vp, _i64, _i64, _int,
+         _vp, _int, _i64, _i64, _i64, _i64, _int, _vp],
+    ),
+    "kvhot_reshape_and_cache_4bit": (
+        _int,
+        [_vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _i64, _int, _vp],
+    ),
+    "kvhot_read_cache_4bit": (
+        _int,
+        [_vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp],
+    ),
+    "kvhot_paged_attention_4bit_workspace_bytes": (
+        _i64,
+        [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int],
+    ),
+    "kvhot_paged_attention_4bit": (
+        _int,
+        [_vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+         _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _int, _vp, _i64, _vp],
+    ),
+}
+
 
 class KvhotError(RuntimeError):
     """A libkvhot entry point returned a nonzero status."""
@@ -102,7 +133,7 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} is missing: build it with `python serving-engine_amd/build.py`"
         )
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **LAYER_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

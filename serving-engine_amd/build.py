@@ -21,7 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libkvhot.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 BUILD_DIR = os.path.join(HERE, "_build")
-SOURCES = ["kvhot_cache.hip", "kvhot_attention.hip"]
+SOURCES = ["kvhot_cache.hip", "kvhot_attention.hip", "kvhot_4bit.hip", "kvhot_rope.hip"]
 TORCH_SOURCE = "kvhot_torch.cpp"
 TORCH_PATH = os.path.join(HERE, "kvhot_torch.so")
 ARCH = "gfx950"

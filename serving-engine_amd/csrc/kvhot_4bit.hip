@@ -1,0 +1,972 @@
+// A KV cache held in 4 bits: the append that quantises, the dense read back
+// and paged attention over it.
+//
+// A value is stored as a code (a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6) of
+// 4 bits, times 2^e with one e for 32 elements of a head: the microscaling
+// format that gfx950 converts in one instruction for two values
+// (v_cvt_scalef32_pk_*_fp4), in both directions, to nearest even.  e is the
+// exponent of the group's largest magnitude less 2, one more where its
+// significand is above 1.75: then no value is off by more than 2^e, half the
+// distance of the two largest codes.  Every value that comes out is a finite
+// number of the type (kScaleLo, kScaleHi); a group that holds an infinity or
+// a NaN comes out as NaN, all 32 of it (scale byte 255).
+//
+// Each (16 tokens, kv head) is one record of 17 * D bytes:
+//   [0, 8D)           K codes, token by token: byte b holds elements 2b, 2b + 1
+//   [8D, 16D)         V codes, pair by pair: byte 16 p + t holds elements
+//                     2p, 2p + 1 of token t
+//   [16D, 16D + D/2)  K scales, group by group: token 4 a + b at 4 b + a
+//   [.., 17D)         V scales, group by group, token by token
+// K rows are the A operand of S^T = K Q^T as they lie.  V's are the A operand
+// of O^T = V^T P^T, whose k index is the token: with a pair's 16 tokens in 16
+// consecutive bytes, a lane loads those of 4 to 8 pairs at once and no V ever
+// goes through LDS.  (Pairs of tokens in a byte would save the permutes after
+// the conversion, but an append would then have to read and write a byte that
+// another token shares.)  The scale orders put what one lane needs into one
+// load.
+#include "kvhot_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+#include <type_traits>
+
+namespace kvhot {
+
+// Smallest and largest scale byte by dtype: half the smallest scale and six
+// times the largest are finite, normal values of the type (fp16: 2^-24, its
+// smallest value, and 49152).
+static int scale_lo(int dtype) { return dtype == KVHOT_F16 ? 104 : 2; }
+static int scale_hi(int dtype) { return dtype == KVHOT_F16 ? 140 : 252; }
+
+static bool head_dim_4bit(int64_t d) { return d == 64 || d == 96 || d == 128 || d == 256; }
+
+// The slot's record, token in it, or nullptr for a slot outside the pool.
+struct Pool4 {
+  char* base;
+  int64_t block_stride;  // bytes
+  int64_t num_slots;
+  int32_t block_size, heads, rec;
+};
+
+__device__ inline char* record_of(const Pool4& p, int64_t slot, int head, int& token) {
+  if (slot < 0 || slot >= p.num_slots) return nullptr;
+  const int64_t b = slot / p.block_size;
+  const int in = static_cast<int>(slot - b * p.block_size);
+  token = in & 15;
+  return p.base + b * p.block_stride + (static_cast<int64_t>(in >> 4) * p.heads + head) * p.rec;
+}
+
+// Eight values of x, as floats.
+template <class T>
+__device__ inline void load8(const typename T::storage* p, bool vec, float (&x)[8]) {
+  if constexpr (sizeof(typename T::storage) == 2) {
+    u32x4 w;
+    if (vec) {
+      w = *reinterpret_cast<const u32x4*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = static_cast<uint32_t>(p[2 * i]) | static_cast<uint32_t>(p[2 * i + 1]) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = T::low_float(w[i]);
+      x[2 * i + 1] = T::high_float(w[i]);
+    }
+  } else {
+    if (vec) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = a[i];
+        x[4 + i] = b[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+  }
+}
+
+// The group's scale byte from a lane's share of it: four neighbouring lanes
+// hold 8 of its 32 values each.
+__device__ inline uint32_t scale_byte(const float (&x)[8], uint32_t lo, uint32_t hi) {
+  // As integers the magnitudes order like the floats, infinities and NaN on top.
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, kWave)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, kWave)));
+  if (top >= 0x7f800000u) return 255;
+  const int e = static_cast<int>(top >> 23) + ((top & 0x7fffffu) > 0x600000u ? 1 : 0) - 2;
+  return static_cast<uint32_t>(min(max(e, static_cast<int>(lo)), static_cast<int>(hi)));
+}
+
+__device__ inline uint32_t quantise8(const float (&x)[8], uint32_t byte) {
+  if (byte == 255) return 0;
+  const float s = __uint_as_float(byte << 23);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+  return w;
+}
+
+// ------------------------------------------------------------------ append --
+
+// A lane quantises 8 elements of one (token, head) row of K or V.
+template <class T, typename SlotT>
+__global__ void __launch_bounds__(256)
+append_4bit_kernel(const typename T::storage* __restrict__ key, const typename T::storage* __restrict__ value,
+                   Pool4 pool, const SlotT* __restrict__ slots, int64_t per_kv, int32_t lanes_per_row, int64_t k_st,
+                   int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec, int v_vec, uint32_t lo, uint32_t hi) {
+  // (Whole quads are in or out: rows are a multiple of 4 lanes.)
+  int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (idx >= 2 * per_kv) return;
+  const bool is_v = idx >= per_kv;
+  if (is_v) idx -= per_kv;
+  const int64_t row = idx / lanes_per_row;
+  const int l = static_cast<int>(idx - row * lanes_per_row);
+  const int64_t t = row / pool.heads;
+  const int h = static_cast<int>(row - t * pool.heads);
+  const int d = lanes_per_row * 8;
+  int tok;
+  char* rec = record_of(pool, static_cast<int64_t>(slots[t]), h, tok);
+  float x[8];
+  load8<T>((is_v ? value + t * v_st + h * v_sh : key + t * k_st + h * k_sh) + l * 8, is_v ? v_vec : k_vec, x);
+  const uint32_t byte = scale_byte(x, lo, hi);
+  const uint32_t w = quantise8(x, byte);
+  if (!rec) return;
+  if (!is_v) {
+    *reinterpret_cast<uint32_t*>(rec + tok * (d / 2) + l * 4) = w;
+    if ((l & 3) == 0) rec[16 * d + (l >> 2) * 16 + (tok & 3) * 4 + (tok >> 2)] = static_cast<char>(byte);
+  } else {
+    char* v = rec + 8 * d + l * 64 + tok;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[16 * i] = static_cast<char>(w >> (8 * i));
+    if ((l & 3) == 0) rec[16 * d + d / 2 + (l >> 2) * 16 + tok] = static_cast<char>(byte);
+  }
+}
+
+// -------------------------------------------------------------- dense read --
+
+// Two values of a code byte, as T's storage type pair (16-bit) or floats.
+template <class T, int I>
+__device__ inline uint32_t pair16(uint32_t w, float s) {
+  if constexpr (std::is_same<T, F16>::value)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, I));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, I));
+}
+
+// The eight codes of w, times the scale, as four packed pairs of M (BF16 or F16).
+template <class M>
+__device__ inline u32x4 codes8(uint32_t w, float s) {
+  return u32x4{pair16<M, 0>(w, s), pair16<M, 1>(w, s), pair16<M, 2>(w, s), pair16<M, 3>(w, s)};
+}
+
+// A scale byte as a float whose exponent it is (the conversions use nothing
+// else of it; 255 makes them return NaN).
+__device__ inline float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// A lane writes 8 elements of one (slot, head) row of K or V.
+template <class T, typename SlotT>
+__global__ void __launch_bounds__(256)
+read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t per_kv, int32_t lanes_per_row,
+                 typename T::storage* __restrict__ key, typename T::storage* __restrict__ value) {
+  int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (idx >= 2 * per_kv) return;
+  const bool is_v = idx >= per_kv;
+  if (is_v) idx -= per_kv;
+  const int64_t row = idx / lanes_per_row;
+  const int l = static_cast<int>(idx - row * lanes_per_row);
+  const int64_t t = row / pool.heads;
+  const int h = static_cast<int>(row - t * pool.heads);
+  const int d = lanes_per_row * 8;
+  int tok = 0;
+  const char* rec = record_of(pool, static_cast<int64_t>(slots[t]), h, tok);
+  uint32_t w = 0, byte = 127;
+  if (rec && !is_v) {
+    w = *reinterpret_cast<const uint32_t*>(rec + tok * (d / 2) + l * 4);
+    byte = static_cast<uint8_t>(rec[16 * d + (l >> 2) * 16 + (tok & 3) * 4 + (tok >> 2)]);
+  } else if (rec) {
+    const uint8_t* v = reinterpret_cast<const uint8_t*>(rec) + 8 * d + l * 64 + tok;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(v[16 * i]) << (8 * i);
+    byte = static_cast<uint8_t>(rec[16 * d + d / 2 + (l >> 2) * 16 + tok]);
+  }
+  const float s = scale_of(byte);
+  typename T::storage* out = (is_v ? value : key) + row * d + l * 8;
+  if constexpr (std::is_same<T, F32>::value) {
+    const u32x4 x = codes8<BF16>(w, s);
+    T::store8(out, f32x4{BF16::low_float(x.x), BF16::high_float(x.x), BF16::low_float(x.y), BF16::high_float(x.y)},
+              f32x4{BF16::low_float(x.z), BF16::high_float(x.z), BF16::low_float(x.w), BF16::high_float(x.w)});
+  } else {
+    *reinterpret_cast<u32x4*>(out) = codes8<T>(w, s);
+  }
+}
+
+// --------------------------------------------------------------- attention --
+
+struct Attn4Args {
+  const void* q;
+  int64_t q_st, q_sh;
+  const char* cache;
+  int64_t block_stride;
+  void* out;
+  int64_t o_st, o_sh;
+  float* lse;
+  int64_t l_st, l_sh;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t *q_lens, *k_lens, *q_starts, *q_offs;
+  int64_t total_query;
+  int32_t num_rows, hq, hkv, group, block_size, num_blocks, causal;
+  float scale;  // times log2(e)
+  int32_t q_vec, o_vec;
+  // the padded grid
+  int32_t q_blocks, parts, part_steps, max_k;
+  float* ws_o;
+  float* ws_lse;
+};
+
+constexpr int kStep = 64;   // keys a wave attends at a time: four records
+constexpr int kWaves4 = 4;  // waves of a work-group, which share out its steps
+
+// One query block of one row and kv head: 16 * MT (query, head) pairs, "m-rows",
+// in the order query by query, against the key steps [step0, step1).
+struct Block4 {
+  int32_t row, head, first;  // first m-row
+  int32_t rows;              // m-rows that exist
+  int32_t q0, off;           // first query token of the row, its position
+  int32_t k_len;
+  int32_t limit;             // keys that any of the m-rows sees
+  int32_t least;             // keys that all of them see
+};
+
+__device__ inline int imin(int a, int b) { return a < b ? a : b; }
+__device__ inline int imax(int a, int b) { return a > b ? a : b; }
+
+// The keys that m-row m of the row sees.
+__device__ inline int sees(const Attn4Args& a, const Block4& b, int m) {
+  if (!a.causal) return b.k_len;
+  const int64_t s = static_cast<int64_t>(b.off) + m / a.group + 1;
+  return static_cast<int>(s < 0 ? 0 : s < b.k_len ? s : b.k_len);
+}
+
+template <int ROWS>
+__device__ inline bool block_of(const Attn4Args& a, int row, int head, int qb, Block4& b) {
+  b.row = row;
+  b.head = head;
+  const int n_q = a.q_lens[row];
+  b.first = qb * ROWS;
+  const int64_t all = static_cast<int64_t>(n_q) * a.group;
+  if (n_q <= 0 || b.first >= all) return false;
+  b.rows = static_cast<int>(all - b.first < ROWS ? all - b.first : ROWS);
+  b.q0 = a.q_starts[row];
+  b.off = a.q_offs[row];
+  b.k_len = imin(imax(a.k_lens[row], 0), a.max_k);
+  // (the table's columns bound what can be read)
+  const int64_t held = a.bt_stride * a.block_size;
+  if (b.k_len > held) b.k_len = static_cast<int>(held);
+  b.limit = sees(a, b, b.first + b.rows - 1);
+  b.least = sees(a, b, b.first);
+  return true;
+}
+
+// Bytes of a step that a lane holds.
+template <int D>
+struct Step4 {
+  static constexpr int NJ = D / 32;
+  uint32_t k[4][NJ];   // codes of token 4 t + (lane & 3), elements 8 * NJ * (lane / 16) on
+  uint32_t ks[2];      // their scales, one byte for each t: of the first and the last element's group
+  u32x4 v[NJ];         // codes of the 16 tokens of record lane / 16, pairs pair_of(lane & 15, c)
+  u32x4 vs[D == 96 ? 3 : 1];  // their scales
+};
+
+// Pair of elements c of A row i of O^T's tiles.  At head_dim 96 an i has one
+// pair in each group, otherwise all of an i's pairs lie in one.
+template <int D>
+__device__ constexpr int pair_of(int i, int c) { return D == 96 ? i + 16 * c : (D / 32) * i + c; }
+
+template <int D>
+__device__ inline void load_step(const Attn4Args& a, const Block4& b, int step, int lane, Step4<D>& s) {
+  constexpr int NJ = Step4<D>::NJ;
+  constexpr int REC = 17 * D;
+  const int i = lane & 15, g = lane >> 4;
+  const int spb = a.block_size >> 4;
+  const int last = (b.limit + 15) / 16 - 1;
+  const int32_t* bt = a.bt + static_cast<int64_t>(b.row) * a.bt_stride;
+  const auto rec = [&](int slice) {
+    slice = imin(slice, last);
+    const int blk = slice / spb;
+    const int id = imin(imax(bt[blk], 0), a.num_blocks - 1);
+    return a.cache + id * a.block_stride + (static_cast<int64_t>(slice - blk * spb) * a.hkv + b.head) * REC;
+  };
+  const char* kr = rec(step * 4 + (i >> 2));
+  const char* vr = rec(step * 4 + g);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const char* p = kr + (4 * t + (i & 3)) * (D / 2) + g * (4 * NJ);
+    if constexpr (NJ == 2) {
+      *reinterpret_cast<u32x2*>(s.k[t]) = *reinterpret_cast<const u32x2*>(p);
+    } else if constexpr (NJ == 3) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) s.k[t][j] = reinterpret_cast<const uint32_t*>(p)[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; j += 4) *reinterpret_cast<u32x4*>(s.k[t] + j) = *reinterpret_cast<const u32x4*>(p + 4 * j);
+    }
+  }
+  const int g0 = (g * NJ) >> 2, g1 = (g * NJ + NJ - 1) >> 2;
+  s.ks[0] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g0 * 16 + (i & 3) * 4);
+  s.ks[1] = s.ks[0];
+  if constexpr (NJ == 3 || NJ == 8) s.ks[1] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g1 * 16 + (i & 3) * 4);
+#pragma unroll
+  for (int c = 0; c < NJ; ++c) s.v[c] = *reinterpret_cast<const u32x4*>(vr + 8 * D + pair_of<D>(i, c) * 16);
+#pragma unroll
+  for (int c = 0; c < (D == 96 ? 3 : 1); ++c)
+    s.vs[c] = *reinterpret_cast<const u32x4*>(vr + 16 * D + D / 2 + (pair_of<D>(i, c) >> 4) * 16);
+}
+
+// Running state of a wave: O^T tiles (tile 2 c + e holds element e of pair c),
+// and for its lane's m-row the reference that exponents are taken against, the
+// score above which it moves, and the lane's share of the sum.
+template <int D, int MT>
+struct State4 {
+  f32x4 o[MT][D / 16];
+  float ref[MT], above[MT], sum[MT];
+};
+
+// A reference that moves goes this far below the score that moved it, and
+// moves again when a score is kRoom above it: probabilities then stay within
+// 2^kRoom (fp16's 65504 included), and those that matter are normal numbers of
+// fp16.
+constexpr float kBelow = 8.0f, kRoom = 15.0f;
+
+template <class M, int NP>
+__device__ inline void split_pair(float a, float b, uint32_t (&p)[NP]) {
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    p[n] = M::pack2(a, b);
+    if (n + 1 < NP) {
+      a -= M::low_float(p[n]);
+      b -= M::high_float(p[n]);
+    }
+  }
+}
+
+// Attends one step.  Q^T is q[tile][part][j]: element 8 (NJ * (lane / 16) + j) on
+// of m-row lane & 15.  MASKED: some m-row does not see all 64 keys.
+template <class M, int NP, int D, int MT, bool MASKED>
+__device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D / 32], const int (&sees)[MT], int base,
+                                   int limit, float scale, int lane, State4<D, MT>& st) {
+  constexpr int NJ = D / 32;
+  const int g = lane >> 4;
+  // S^T: row 4 g + r of tile t is token 4 t + r of record g.
+  f32x4 sc[MT][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sc[m][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const bool second = NJ == 8 ? j >= 4 : NJ == 3 ? ((g * 3 + j) >> 2) != ((g * 3) >> 2) : false;
+      const uint32_t sw = second ? s.ks[1] : s.ks[0];
+      const u32x4 k = codes8<M>(s.k[t][j], scale_of((sw >> (8 * t)) & 255));
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) sc[m][t] = M::mfma(k, q[m][n][j], sc[m][t]);
+    }
+  }
+  // Probabilities: lane (n, g) holds m-row n's for the 16 tokens of record g, the
+  // B operand of O^T's two products of 32 tokens.
+  u32x4 p[MT][NP][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = sc[m][t][r] * scale;
+        if (MASKED && base + 16 * g + 4 * t + r >= sees[m]) x = -INFINITY;
+        sc[m][t][r] = x;
+        top = fmaxf(top, x);
+      }
+    if (__any(top > st.above[m])) {
+      top = fmaxf(top, __shfl_xor(top, 16, kWave));
+      top = fmaxf(top, __shfl_xor(top, 32, kWave));
+      if (top > st.above[m]) {
+        const float ref = top - kBelow;
+        const float f = st.above[m] == -INFINITY ? 0.0f : F32::exp2(st.ref[m] - ref);
+        st.ref[m] = ref;
+        st.above[m] = ref + kRoom;
+        st.sum[m] *= f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) st.o[m][c][r] *= f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const float x = BF16::exp2(sc[m][t][r] - st.ref[m]), y = BF16::exp2(sc[m][t][r + 1] - st.ref[m]);
+        st.sum[m] += x + y;
+        uint32_t w[NP];
+        split_pair<M, NP>(x, y, w);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) p[m][n][t >> 1][(t & 1) * 2 + (r >> 1)] = w[n];
+      }
+  }
+  // V's scales: one float a token.  In a masked step a NaN may belong to a key
+  // that some m-row does not see, whose probability of 0 it would turn into NaN
+  // too: it is taken out here and put into the m-rows that see it below.  What
+  // lies behind the last key that any of them sees may be anything: its scales
+  // are 1.
+  constexpr int NS = D == 96 ? 3 : 1;
+  u32x4 vs[NS];
+  uint32_t bad[NS];
+#pragma unroll
+  for (int c = 0; c < NS; ++c) {
+    vs[c] = s.vs[c];
+    bad[c] = 0;
+    if (MASKED) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const uint32_t sh = 8 * (t & 3);
+        const bool seen = base + 16 * g + t < limit, nan = ((vs[c][t >> 2] >> sh) & 255) == 255;
+        if (seen && nan) bad[c] |= 1u << t;
+        if (!seen || nan) vs[c][t >> 2] = (vs[c][t >> 2] & ~(255u << sh)) | 127u << sh;
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < NJ; ++c) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      u32x4 lo, hi;  // elements 2 pair, 2 pair + 1 of tokens 8 u .. 8 u + 7
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t code = s.v[c][2 * u + w], sb = vs[NS == 3 ? c : 0][2 * u + w];
+        const uint32_t a0 = pair16<M, 0>(code, scale_of(sb & 255)), a1 = pair16<M, 1>(code, scale_of((sb >> 8) & 255)),
+                       a2 = pair16<M, 2>(code, scale_of((sb >> 16) & 255)), a3 = pair16<M, 3>(code, scale_of(sb >> 24));
+        lo[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x05040100);
+        lo[2 * w + 1] = __builtin_amdgcn_perm(a3, a2, 0x05040100);
+        hi[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x07060302);
+        hi[2 * w + 1] = __builtin_amdgcn_perm(a3, a2, 0x07060302);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = NP - 1; n >= 0; --n) {
+          st.o[m][2 * c] = M::mfma(lo, p[m][n][u], st.o[m][2 * c]);
+          st.o[m][2 * c + 1] = M::mfma(hi, p[m][n][u], st.o[m][2 * c + 1]);
+        }
+    }
+  }
+  if constexpr (MASKED) {
+    bool any = false;
+#pragma unroll
+    for (int c = 0; c < NS; ++c) any |= bad[c] != 0;
+    if (__any(any)) {
+      // How many NaN of its elements each m-row sees, as one more product.
+      const uint32_t one = M::pack2(1.0f, 1.0f);
+#pragma unroll
+      for (int c = 0; c < NS; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          f32x4 n{0, 0, 0, 0};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            u32x4 x, y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int t = 8 * u + 2 * w, key = base + 16 * g + t;
+              x[w] = ((bad[c] >> t) & 1 ? one & 0xffffu : 0) | ((bad[c] >> (t + 1)) & 1 ? one & 0xffff0000u : 0);
+              y[w] = (key < sees[m] ? one & 0xffffu : 0) | (key + 1 < sees[m] ? one & 0xffff0000u : 0);
+            }
+            n = M::mfma(x, y, n);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n[r] > 0) {
+#pragma unroll
+              for (int e = 0; e < D / 16; ++e)
+                if (NS == 1 || (e >> 1) == c) st.o[m][e][r] = __builtin_nanf("");
+            }
+        }
+    }
+  }
+}
+
+// Adds the state of another wave, read from LDS, to this wave's.
+template <int D, int MT>
+__device__ inline void join(State4<D, MT>& a, const float* lds, int lane) {
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const float* p = lds + m * (D / 16 * 4 + 3) * kWave + lane;
+    const float ref = p[0], above = p[kWave], sum = p[2 * kWave];
+    float fa = 1.0f, fb = 1.0f;
+    if (above == -INFINITY) {  // no finite score there: its sums are 0, or NaN
+      fb = 0.0f;
+    } else if (a.above[m] == -INFINITY) {
+      fa = 0.0f;
+      a.ref[m] = ref;
+      a.above[m] = above;
+    } else if (ref > a.ref[m]) {
+      fa = F32::exp2(a.ref[m] - ref);
+      a.ref[m] = ref;
+      a.above[m] = above;
+    } else {
+      fb = F32::exp2(ref - a.ref[m]);
+    }
+    a.sum[m] = a.sum[m] * fa + sum * fb;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) a.o[m][c][r] = a.o[m][c][r] * fa + p[(3 + c * 4 + r) * kWave] * fb;
+  }
+}
+
+template <int D, int MT>
+__device__ inline void park(const State4<D, MT>& a, float* lds, int lane) {
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float* p = lds + m * (D / 16 * 4 + 3) * kWave + lane;
+    p[0] = a.ref[m];
+    p[kWave] = a.above[m];
+    p[2 * kWave] = a.sum[m];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[(3 + c * 4 + r) * kWave] = a.o[m][c][r];
+  }
+}
+
+template <int D, int MT>
+constexpr int parked() { return MT * (D / 16 * 4 + 3) * kWave; }
+
+template <class IO, class M, int NP, int D, int MT>
+__global__ void __launch_bounds__(64 * kWaves4)
+attn_4bit_kernel(Attn4Args a) {
+  constexpr int NJ = D / 32, ROWS = 16 * MT;
+  __shared__ float lds[kWaves4 / 2 * parked<D, MT>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t u = blockIdx.x;
+  const int head = static_cast<int>(u % a.hkv);
+  u /= a.hkv;
+  const int part = static_cast<int>(u % a.parts);
+  u /= a.parts;
+  const int qb = static_cast<int>(u % a.q_blocks);
+  const int row = static_cast<int>(u / a.q_blocks);
+  Block4 b;
+  if (!block_of<ROWS>(a, row, head, qb, b)) return;
+  const int steps = (b.limit + kStep - 1) / kStep;
+  const int step0 = part * a.part_steps, step1 = imin(steps, step0 + a.part_steps);
+  if (part > 0 && step0 >= steps) return;
+  const bool whole = steps <= a.part_steps;
+  const int n = lane & 15, g = lane >> 4;
+
+  u32x4 q[MT][NP][NJ];
+  int lim[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int mr = b.first + 16 * m + n;
+    const bool there = 16 * m + n < b.rows;
+    const int tok = b.q0 + mr / a.group;
+    lim[m] = there ? sees(a, b, mr) : b.limit;
+    const bool ok = there && tok >= 0 && tok < a.total_query;
+    const typename IO::storage* src = static_cast<const typename IO::storage*>(a.q) +
+                                      (ok ? tok * a.q_st + (b.head * a.group + mr % a.group) * a.q_sh : 0) + g * NJ * 8;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      float x[8];
+      if (ok) {
+        load8<IO>(src + 8 * j, a.q_vec, x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[NP];
+        split_pair<M, NP>(x[2 * i], x[2 * i + 1], w);
+#pragma unroll
+        for (int k = 0; k < NP; ++k) q[m][k][j][i] = w[k];
+      }
+    }
+  }
+  State4<D, MT> st;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    st.ref[m] = 0;
+    st.above[m] = -INFINITY;
+    st.sum[m] = 0;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) st.o[m][c] = f32x4{0, 0, 0, 0};
+  }
+  if (step0 + wave < step1) {
+    Step4<D> cur;
+    load_step<D>(a, b, step0 + wave, lane, cur);
+    for (int s = step0 + wave; s < step1; s += kWaves4) {
+      Step4<D> next;
+      const bool more = s + kWaves4 < step1;
+      if (more) load_step<D>(a, b, s + kWaves4, lane, next);
+      if (s * kStep + kStep <= b.least)
+        attend_step<M, NP, D, MT, false>(cur, q, lim, s * kStep, b.limit, a.scale, lane, st);
+      else
+        attend_step<M, NP, D, MT, true>(cur, q, lim, s * kStep, b.limit, a.scale, lane, st);
+      if (more) cur = next;
+    }
+  }
+  // The waves' states, joined in LDS: 2 and 3 into 0 and 1, then 1 into 0.
+  if (wave >= 2) park<D, MT>(st, lds + (wave - 2) * parked<D, MT>(), lane);
+  __syncthreads();
+  if (wave < 2) join<D, MT>(st, lds + wave * parked<D, MT>(), lane);
+  __syncthreads();
+  if (wave == 1) park<D, MT>(st, lds, lane);
+  __syncthreads();
+  if (wave != 0) return;
+  join<D, MT>(st, lds, lane);
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float sum = st.sum[m];
+    sum += __shfl_xor(sum, 16, kWave);
+    sum += __shfl_xor(sum, 32, kWave);
+    if (16 * m + n >= b.rows) continue;
+    const int mr = b.first + 16 * m + n;
+    const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
+    const float inv = sum == 0 ? 0.0f : 1.0f / sum;  // no key seen: 0
+    const float lse2 = sum == 0 ? -INFINITY : st.ref[m] + F32::log2(sum);
+    float x[4][D / 16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) x[r][e] = st.o[m][e][r] * inv;
+    if (whole) {
+      if (tok < 0 || tok >= a.total_query) continue;
+      typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + hd * a.o_sh;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 4 * g + r;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[2 * pair_of<D>(i, e >> 1) + (e & 1)] = IO::from_float(x[r][e]);
+      }
+      if (a.lse && g == 0) a.lse[tok * a.l_st + hd * a.l_sh] = lse2 * kLn2;
+    } else {
+      const int64_t w = ((static_cast<int64_t>(row) * a.q_blocks + qb) * a.parts + part) * a.hkv + head;
+      float* o = a.ws_o + (w * ROWS + 16 * m + n) * D;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 4 * g + r;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[2 * pair_of<D>(i, e >> 1) + (e & 1)] = x[r][e];
+      }
+      if (g == 0) a.ws_lse[w * ROWS + 16 * m + n] = lse2;
+    }
+  }
+}
+
+// Joins the parts of the query blocks that were cut: one wave an m-row.
+template <class IO, int D, int ROWS>
+__global__ void __launch_bounds__(256)
+merge_4bit_kernel(Attn4Args a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t u = blockIdx.x;
+  const int head = static_cast<int>(u % a.hkv);
+  u /= a.hkv;
+  const int qb = static_cast<int>(u % a.q_blocks);
+  const int row = static_cast<int>(u / a.q_blocks);
+  Block4 b;
+  if (!block_of<ROWS>(a, row, head, qb, b)) return;
+  const int steps = (b.limit + kStep - 1) / kStep;
+  const int parts = (steps + a.part_steps - 1) / a.part_steps;
+  if (parts <= 1) return;
+  for (int m = wave; m < b.rows; m += 4) {
+    const int mr = b.first + m;
+    const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
+    if (tok < 0 || tok >= a.total_query) continue;
+    const int64_t w0 = (static_cast<int64_t>(row) * a.q_blocks + qb) * a.parts * a.hkv + head;
+    float top = -INFINITY;
+    for (int p = 0; p < parts; ++p) {
+      const float l = a.ws_lse[(w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m];
+      top = l > top || l != l ? l : top;
+    }
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0, x[(D + 63) / 64] = {};
+    for (int p = 0; p < parts; ++p) {
+      const int64_t w = ((w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m);
+      const float f = F32::exp2(a.ws_lse[w] - ref);
+      sum += f;
+#pragma unroll
+      for (int i = 0; i < (D + 63) / 64; ++i)
+        if (i * 64 + lane < D) x[i] += f * a.ws_o[w * D + i * 64 + lane];
+    }
+    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+    typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + hd * a.o_sh;
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i)
+      if (i * 64 + lane < D) o[i * 64 + lane] = IO::from_float(x[i] * inv);
+    if (a.lse && lane == 0) a.lse[tok * a.l_st + hd * a.l_sh] = sum == 0 ? -INFINITY : (ref + F32::log2(sum)) * kLn2;
+  }
+}
+
+// Split of a call: the query block's m-rows, key steps of a part, parts.
+struct Split4 {
+  int32_t mt, q_blocks, parts, part_steps;
+  int64_t ws_bytes;
+};
+
+static Split4 split_4bit(int64_t rows, int64_t max_q, int64_t max_k, int64_t group, int64_t hkv, int64_t d, int dtype) {
+  Split4 s;
+  s.mt = max_q * group > 16 && dtype != KVHOT_F32 && d <= 128 ? 2 : 1;
+  s.q_blocks = static_cast<int32_t>((max_q * group + 16 * s.mt - 1) / (16 * s.mt));
+  const int64_t steps = (max_k + kStep - 1) / kStep;
+  // Work-groups enough for four on each of 256 CUs, with two steps a wave at
+  // least.
+  const int64_t blocks = rows * s.q_blocks * hkv;
+  int64_t parts = std::max<int64_t>(1, (1024 + blocks - 1) / blocks);
+  int64_t per = std::max<int64_t>((steps + parts - 1) / parts, 2 * kWaves4);
+  s.part_steps = static_cast<int32_t>(std::max<int64_t>(per, 1));
+  s.parts = static_cast<int32_t>(std::max<int64_t>((steps + per - 1) / per, 1));
+  s.ws_bytes = s.parts > 1 ? blocks * s.parts * 16 * s.mt * (d + 1) * 4 : 0;
+  return s;
+}
+
+}  // namespace kvhot
+
+using namespace kvhot;
+
+static int check_pool(const char* what, const void* cache, int64_t block_stride, int64_t heads, int64_t d,
+                      int64_t block_size, int64_t num_blocks) {
+  const std::string w(what);
+  if (heads <= 0 || d <= 0 || block_size <= 0 || num_blocks < 0) return set_error(KVHOT_EINVAL, w + ": bad sizes");
+  if (!head_dim_4bit(d)) return set_error(KVHOT_EUNSUPPORTED, w + ": head_dim must be 64, 96, 128 or 256");
+  if (block_size % 16 != 0) return set_error(KVHOT_EUNSUPPORTED, w + ": block_size must be a multiple of 16");
+  if (num_blocks > 0x7fffffff || block_size > (1 << 20) || heads > (1 << 16))
+    return set_error(KVHOT_EUNSUPPORTED, w + ": sizes beyond the kernels' range");
+  if (!cache && num_blocks > 0) return set_error(KVHOT_EINVAL, w + ": null pointer");
+  if (reinterpret_cast<uintptr_t>(cache) % 16 || block_stride % 16)
+    return set_error(KVHOT_EINVAL, w + ": the cache and its block stride must be multiples of 16 bytes");
+  if (num_blocks > 1 && block_stride < block_size / 16 * heads * 17 * d)
+    return set_error(KVHOT_EINVAL, w + ": blocks overlap");
+  return 0;
+}
+
+static Pool4 pool_of(const void* cache, int64_t block_stride, int64_t heads, int64_t d, int64_t block_size,
+                     int64_t num_blocks) {
+  return Pool4{const_cast<char*>(static_cast<const char*>(cache)), block_stride, num_blocks * block_size,
+               static_cast<int32_t>(block_size), static_cast<int32_t>(heads), static_cast<int32_t>(17 * d)};
+}
+
+static bool aligned(const void* p, int64_t es, int64_t unit, std::initializer_list<int64_t> strides) {
+  if (reinterpret_cast<uintptr_t>(p) % unit) return false;
+  for (int64_t s : strides)
+    if (s * es % unit) return false;
+  return true;
+}
+
+extern "C" int kvhot_reshape_and_cache_4bit(
+    const void* key, const int64_t key_strides[3], const void* value, const int64_t value_strides[3], void* cache,
+    int64_t block_stride_bytes, const void* slot_mapping, int slot_is_int64, int64_t num_tokens, int64_t num_kv_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks, int dtype, void* stream) {
+  clear_error();
+  const int64_t es = dtype_size(dtype);
+  if (es == 0) return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: bad dtype");
+  if (num_tokens < 0) return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: bad sizes");
+  if (int e = check_pool("reshape_and_cache_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
+    return e;
+  if (num_tokens == 0 || num_blocks == 0) return 0;
+  if (!key || !value || !slot_mapping || !key_strides || !value_strides)
+    return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: null pointer");
+  if (key_strides[2] != 1 || value_strides[2] != 1)
+    return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: head_dim must be the innermost, unit-stride dim");
+  if (reinterpret_cast<uintptr_t>(key) % es || reinterpret_cast<uintptr_t>(value) % es)
+    return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: misaligned tensors");
+  const int64_t per_kv = num_tokens * num_kv_heads * (head_dim / 8);
+  const int64_t groups = (2 * per_kv + 255) / 256;
+  if (groups > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "reshape_and_cache_4bit: too many tokens");
+  const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
+  const int kv = aligned(key, es, 16, {key_strides[0], key_strides[1]});
+  const int vv = aligned(value, es, 16, {value_strides[0], value_strides[1]});
+#define KVHOT_GO(T, S)                                                                                               \
+  hipLaunchKernelGGL((append_4bit_kernel<T, S>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0,                   \
+                     static_cast<hipStream_t>(stream), static_cast<const T::storage*>(key),                           \
+                     static_cast<const T::storage*>(value), pool, static_cast<const S*>(slot_mapping), per_kv,        \
+                     static_cast<int32_t>(head_dim / 8), key_strides[0], key_strides[1], value_strides[0],            \
+                     value_strides[1], kv, vv, scale_lo(dtype), scale_hi(dtype))
+  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {
+    case KVHOT_F32 * 2: KVHOT_GO(F32, int32_t); break;
+    case KVHOT_F32 * 2 + 1: KVHOT_GO(F32, int64_t); break;
+    case KVHOT_F16 * 2: KVHOT_GO(F16, int32_t); break;
+    case KVHOT_F16 * 2 + 1: KVHOT_GO(F16, int64_t); break;
+    case KVHOT_BF16 * 2: KVHOT_GO(BF16, int32_t); break;
+    default: KVHOT_GO(BF16, int64_t); break;
+  }
+#undef KVHOT_GO
+  return launch_status("reshape_and_cache_4bit");
+}
+
+extern "C" int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_bytes, const void* slots, int slot_is_int64,
+                                     int64_t num_slots, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                     int64_t num_blocks, void* key, void* value, int dtype, void* stream) {
+  clear_error();
+  if (dtype_size(dtype) == 0) return set_error(KVHOT_EINVAL, "read_cache_4bit: bad dtype");
+  if (num_slots < 0) return set_error(KVHOT_EINVAL, "read_cache_4bit: bad sizes");
+  if (int e = check_pool("read_cache_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
+    return e;
+  if (num_slots == 0) return 0;
+  if (!key || !value || !slots) return set_error(KVHOT_EINVAL, "read_cache_4bit: null pointer");
+  if (reinterpret_cast<uintptr_t>(key) % 16 || reinterpret_cast<uintptr_t>(value) % 16)
+    return set_error(KVHOT_EINVAL, "read_cache_4bit: misaligned tensors");
+  const int64_t per_kv = num_slots * num_kv_heads * (head_dim / 8);
+  const int64_t groups = (2 * per_kv + 255) / 256;
+  if (groups > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "read_cache_4bit: too many slots");
+  const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
+#define KVHOT_GO(T, S)                                                                                             \
+  hipLaunchKernelGGL((read_4bit_kernel<T, S>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0,                   \
+                     static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), per_kv,                  \
+                     static_cast<int32_t>(head_dim / 8), static_cast<T::storage*>(key), static_cast<T::storage*>(value))
+  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {
+    case KVHOT_F32 * 2: KVHOT_GO(F32, int32_t); break;
+    case KVHOT_F32 * 2 + 1: KVHOT_GO(F32, int64_t); break;
+    case KVHOT_F16 * 2: KVHOT_GO(F16, int32_t); break;
+    case KVHOT_F16 * 2 + 1: KVHOT_GO(F16, int64_t); break;
+    case KVHOT_BF16 * 2: KVHOT_GO(BF16, int32_t); break;
+    default: KVHOT_GO(BF16, int64_t); break;
+  }
+#undef KVHOT_GO
+  return launch_status("read_cache_4bit");
+}
+
+static int check_attention(int64_t rows, int64_t total, int64_t max_q, int64_t max_k, int64_t hq, int64_t hkv, int64_t d,
+                           int dtype) {
+  if (rows < 0 || total < 0 || max_q < 0 || max_k < 0 || hq <= 0 || hkv <= 0 || d <= 0)
+    return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
+  if (hq % hkv != 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: num_q_heads must be a multiple of num_kv_heads");
+  if (dtype_size(dtype) == 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad dtype");
+  if (!head_dim_4bit(d)) return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: head_dim must be 64, 96, 128 or 256");
+  if (max_k > 0x7fffff00 || max_q > 0x7fffff00 || hq > (1 << 16) || max_q * (hq / hkv) > 0x7fffff00)
+    return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: sizes beyond the kernels' range");
+  return 0;
+}
+
+extern "C" int64_t kvhot_paged_attention_4bit_workspace_bytes(int64_t num_rows, int64_t total_query, int64_t max_q_len,
+                                                              int64_t max_k_len, int64_t num_q_heads,
+                                                              int64_t num_kv_heads, int64_t head_dim, int dtype) {
+  clear_error();
+  if (int e = check_attention(num_rows, total_query, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
+    return e;
+  if (num_rows == 0 || total_query == 0 || max_q_len == 0) return 0;
+  return split_4bit(num_rows, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim, dtype).ws_bytes;
+}
+
+namespace {
+
+template <class IO, class M, int NP, int D, int MT>
+int launch_4bit(const Attn4Args& a, int64_t rows, hipStream_t s) {
+  const int64_t blocks = rows * a.q_blocks * a.hkv;
+  if (blocks * a.parts > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
+  hipLaunchKernelGGL((attn_4bit_kernel<IO, M, NP, D, MT>), dim3(static_cast<uint32_t>(blocks * a.parts)),
+                     dim3(64 * kWaves4), 0, s, a);
+  if (int e = launch_status("paged_attention_4bit")) return e;
+  if (a.parts > 1) {
+    hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, s, a);
+    return launch_status("paged_attention_4bit merge");
+  }
+  return 0;
+}
+
+template <class IO, class M, int NP, int D>
+int launch_4bit(const Attn4Args& a, int mt, int64_t rows, hipStream_t s) {
+  if constexpr (NP == 1 && D <= 128)
+    if (mt == 2) return launch_4bit<IO, M, NP, D, 2>(a, rows, s);
+  return launch_4bit<IO, M, NP, D, 1>(a, rows, s);
+}
+
+template <class IO, class M, int NP>
+int launch_4bit(const Attn4Args& a, int64_t d, int mt, int64_t rows, hipStream_t s) {
+  switch (d) {
+    case 64: return launch_4bit<IO, M, NP, 64>(a, mt, rows, s);
+    case 96: return launch_4bit<IO, M, NP, 96>(a, mt, rows, s);
+    case 128: return launch_4bit<IO, M, NP, 128>(a, mt, rows, s);
+    default: return launch_4bit<IO, M, NP, 256>(a, mt, rows, s);
+  }
+}
+
+}  // namespace
+
+extern "C" int kvhot_paged_attention_4bit(
+    const void* q, const int64_t q_strides[3], const void* cache, int64_t block_stride_bytes, void* out,
+    const int64_t out_strides[3], float* lse, const int64_t lse_strides[2], const int32_t* block_table,
+    int64_t bt_row_stride, const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_starts,
+    const int32_t* q_pos_offsets, int64_t num_rows, int64_t total_query, int64_t max_q_len, int64_t max_k_len,
+    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks, float scale,
+    int attn_flags, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (int e = check_attention(num_rows, total_query, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
+    return e;
+  if (int e = check_pool("paged_attention_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
+    return e;
+  if (attn_flags & ~KVHOT_CAUSAL) return set_error(KVHOT_EINVAL, "paged_attention_4bit: unknown attn_flags");
+  if (num_rows == 0 || total_query == 0 || max_q_len == 0) return 0;
+  if (!q || !out || !q_strides || !out_strides || !q_lens || !k_lens || !q_starts || !q_pos_offsets ||
+      (lse && !lse_strides) || (!block_table && bt_row_stride > 0 && max_k_len > 0))
+    return set_error(KVHOT_EINVAL, "paged_attention_4bit: null pointer");
+  if (q_strides[2] != 1 || out_strides[2] != 1)
+    return set_error(KVHOT_EINVAL, "paged_attention_4bit: head_dim must be the innermost, unit-stride dim");
+  if (bt_row_stride < 0 || num_rows > 0x7fffffff) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
+  if (num_blocks == 0 && max_k_len > 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: keys but no blocks");
+  const Split4 sp = split_4bit(num_rows, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim, dtype);
+  if (sp.ws_bytes > 0 && (!workspace || workspace_bytes < sp.ws_bytes))
+    return set_error(KVHOT_EWORKSPACE, "paged_attention_4bit: workspace missing or too small");
+  const int64_t es = dtype_size(dtype);
+  Attn4Args a;
+  a.q = q;
+  a.q_st = q_strides[0];
+  a.q_sh = q_strides[1];
+  a.cache = static_cast<const char*>(cache);
+  a.block_stride = block_stride_bytes;
+  a.out = out;
+  a.o_st = out_strides[0];
+  a.o_sh = out_strides[1];
+  a.lse = lse;
+  a.l_st = lse ? lse_strides[0] : 0;
+  a.l_sh = lse ? lse_strides[1] : 0;
+  a.bt = block_table;
+  a.bt_stride = bt_row_stride;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.q_starts = q_starts;
+  a.q_offs = q_pos_offsets;
+  a.total_query = total_query;
+  a.num_rows = static_cast<int32_t>(num_rows);
+  a.hq = static_cast<int32_t>(num_q_heads);
+  a.hkv = static_cast<int32_t>(num_kv_heads);
+  a.group = a.hq / a.hkv;
+  a.block_size = static_cast<int32_t>(block_size);
+  a.num_blocks = static_cast<int32_t>(num_blocks);
+  a.causal = attn_flags & KVHOT_CAUSAL;
+  a.scale = scale * kLog2e;
+  a.q_vec = aligned(q, es, 16, {q_strides[0], q_strides[1]});
+  a.o_vec = aligned(out, es, 16, {out_strides[0], out_strides[1]});
+  a.q_blocks = sp.q_blocks;
+  a.parts = sp.parts;
+  a.part_steps = sp.part_steps;
+  a.max_k = static_cast<int32_t>(max_k_len);
+  a.ws_o = static_cast<float*>(workspace);
+  a.ws_lse = a.ws_o ? a.ws_o + num_rows * sp.q_blocks * sp.parts * num_kv_heads * 16 * sp.mt * head_dim : nullptr;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case KVHOT_F32: return launch_4bit<F32, BF16, 3>(a, head_dim, sp.mt, num_rows, s);
+    case KVHOT_F16: return launch_4bit<F16, F16, 1>(a, head_dim, sp.mt, num_rows, s);
+    default: return launch_4bit<BF16, BF16, 1>(a, head_dim, sp.mt, num_rows, s);
+  }
+}

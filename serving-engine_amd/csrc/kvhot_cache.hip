@@ -325,3 +325,142 @@ extern "C" int kvhot_build_slot_mapping(const int32_t* block_table,
                      total_query, slot_mapping, positions);
   return launch_status("build_slot_mapping");
 }
+
+// ------------------------------------------------------------ block tables --
+
+namespace kvhot {
+
+constexpr int kTableRows = 64;  // rows of a work-group: one wave scans their lengths
+
+// Work-group x has rows [64 x, 64 x + 64); its y parts share out the rows' new
+// blocks and tokens, flattened.  What the rows before them take is summed
+// again by every work-group: a second launch, or a work-group waiting for
+// another, costs more than reading 8 bytes a row.
+__global__ void __launch_bounds__(256)
+block_tables_kernel(int32_t* __restrict__ bt, int64_t bt_stride, const int32_t* __restrict__ prior_lens,
+                    const int32_t* __restrict__ q_lens, const int32_t* __restrict__ free_blocks, int64_t num_free,
+                    int64_t num_rows, int64_t total, int32_t block_size, int32_t* __restrict__ q_starts,
+                    int32_t* __restrict__ k_lens, int64_t* __restrict__ slots, int64_t* __restrict__ positions,
+                    int32_t* __restrict__ taken) {
+  __shared__ int64_t before[2][4];
+  __shared__ int64_t tok_at[kTableRows + 1], new_at[kTableRows + 1];  // first token and new block of each row
+  __shared__ int32_t prior[kTableRows], held[kTableRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTableRows;
+  const auto blocks = [&](int64_t len) { return (len + block_size - 1) / block_size; };
+  int64_t tokens = 0, fresh = 0;
+  for (int64_t r = threadIdx.x; r < first; r += 256) {
+    const int64_t p = max(prior_lens[r], 0), q = max(q_lens[r], 0);
+    tokens += q;
+    fresh += blocks(p + q) - blocks(p);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    tokens += __shfl_xor(tokens, o, kWave);
+    fresh += __shfl_xor(fresh, o, kWave);
+  }
+  if (lane == 0) {
+    before[0][wave] = tokens;
+    before[1][wave] = fresh;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int64_t r = first + lane;
+    int64_t p = 0, q = 0;
+    if (r < num_rows) {
+      p = max(prior_lens[r], 0);
+      q = max(q_lens[r], 0);
+    }
+    const int64_t h = blocks(p), f = blocks(p + q) - h;
+    int64_t ends = q, new_ends = f;  // inclusive sums
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(ends, o, kWave), y = __shfl_up(new_ends, o, kWave);
+      if (lane >= o) {
+        ends += x;
+        new_ends += y;
+      }
+    }
+    ends += before[0][0] + before[0][1] + before[0][2] + before[0][3];
+    new_ends += before[1][0] + before[1][1] + before[1][2] + before[1][3];
+    tok_at[lane + 1] = ends;
+    new_at[lane + 1] = new_ends;
+    if (lane == 0) {
+      tok_at[0] = ends - q;
+      new_at[0] = new_ends - f;
+    }
+    prior[lane] = static_cast<int32_t>(p);
+    held[lane] = static_cast<int32_t>(h);
+    if (r < num_rows && blockIdx.y == 0) {
+      q_starts[r] = static_cast<int32_t>(ends - q);
+      k_lens[r] = static_cast<int32_t>(p + q);
+    }
+  }
+  __syncthreads();
+  // The row that item i belongs to: the last whose first item is at or before i
+  // (rows without items have the next one's).
+  const auto row_of = [](const int64_t* at, int64_t i) {
+    int lo = 0;
+#pragma unroll
+    for (int o = kTableRows / 2; o > 0; o >>= 1)
+      if (at[lo + o] <= i) lo += o;
+    return lo;
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.y) * 256;
+  const int64_t at = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x;
+  for (int64_t i = new_at[0] + at; i < new_at[kTableRows]; i += step) {
+    const int j = row_of(new_at, i);
+    const int64_t col = held[j] + (i - new_at[j]);
+    if (col < bt_stride) bt[(first + j) * bt_stride + col] = i < num_free ? free_blocks[i] : 0;
+  }
+  const int64_t end = tok_at[kTableRows] < total ? tok_at[kTableRows] : total;
+  for (int64_t t = tok_at[0] + at; t < end; t += step) {
+    const int j = row_of(tok_at, t);
+    const int64_t pos = prior[j] + (t - tok_at[j]);
+    const int64_t col = pos / block_size, i = new_at[j] + (col - held[j]);
+    int32_t id = -1;
+    if (col < bt_stride) {
+      if (col < held[j])
+        id = bt[(first + j) * bt_stride + col];
+      else if (i < num_free)
+        id = free_blocks[i];
+    }
+    slots[t] = id < 0 ? -1 : static_cast<int64_t>(id) * block_size + (pos - col * block_size);
+    positions[t] = pos;
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    for (int64_t t = tok_at[kTableRows] + at; t < total; t += step) {
+      slots[t] = -1;
+      positions[t] = 0;
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) *taken = static_cast<int32_t>(new_at[kTableRows]);
+  }
+}
+
+}  // namespace kvhot
+
+extern "C" int kvhot_build_block_tables(int32_t* block_table, int64_t bt_row_stride, const int32_t* prior_lens,
+                                        const int32_t* q_lens, const int32_t* free_blocks, int64_t num_free,
+                                        int64_t num_rows, int64_t total_query, int64_t max_q_len, int64_t block_size,
+                                        int32_t* q_starts, int32_t* k_lens, int64_t* slot_mapping, int64_t* positions,
+                                        int32_t* blocks_taken, void* stream) {
+  clear_error();
+  if (num_rows < 0 || total_query < 0 || max_q_len < 0 || block_size <= 0 || bt_row_stride < 0 || num_free < 0)
+    return set_error(KVHOT_EINVAL, "build_block_tables: bad sizes");
+  if (num_rows > 0x7fffffff || total_query > 0x7fffffff || block_size > 0x7fffffff || num_free > 0x7fffffff)
+    return set_error(KVHOT_EUNSUPPORTED, "build_block_tables: sizes beyond int32");
+  if (num_rows == 0) return set_error(KVHOT_EINVAL, "build_block_tables: no rows");
+  if (!prior_lens || !q_lens || !q_starts || !k_lens || !blocks_taken || (bt_row_stride > 0 && !block_table) ||
+      (num_free > 0 && !free_blocks) || (total_query > 0 && (!slot_mapping || !positions)))
+    return set_error(KVHOT_EINVAL, "build_block_tables: null pointer");
+  const int64_t groups = (num_rows + kTableRows - 1) / kTableRows;
+  // Four tokens a thread for the longest group there can be, and no more
+  // work-groups than fill the device.
+  const int64_t longest = max_q_len > 16384 ? 64 * 16384 : 64 * max_q_len;
+  const int64_t y = longest / 1024 < 1 ? 1 : longest / 1024 > 256 ? 256 : longest / 1024;
+  hipLaunchKernelGGL(block_tables_kernel, dim3(static_cast<uint32_t>(groups), static_cast<uint32_t>(y)), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), block_table, bt_row_stride, prior_lens, q_lens, free_blocks,
+                     num_free, num_rows, total_query, static_cast<int32_t>(block_size), q_starts, k_lens, slot_mapping,
+                     positions, blocks_taken);
+  return launch_status("build_block_tables");
+}

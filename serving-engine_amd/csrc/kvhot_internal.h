@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/kvhot.h"
+#include "../../include/kvhot_layer.h"
 
 namespace kvhot {
 

@@ -28,10 +28,32 @@ import torch
 from . import _lib
 from .block import BLOCK_SIZE
 from . import paged_attention_kernel as _attention
+from .kv_cache_4bit import _PagedKVCache4Bit, paged_flash_attention_4bit
 from .paged_attention_kernel import build_paged_batch_metadata, paged_flash_attention
 from .request import RequestPhase
 
 PAGED_HIP_ATTN_IMPL = "paged|hip"
+
+
+def _checked_pairs(src_block_ids, dst_block_ids, num_blocks, validate, device):
+    """copy_blocks' ids as int64 tensors on the device, checked as it says;
+    (None, None) for no pairs."""
+    src = torch.as_tensor(src_block_ids, dtype=torch.int64)
+    dst = torch.as_tensor(dst_block_ids, dtype=torch.int64)
+    if src.shape != dst.shape or src.dim() != 1:
+        raise ValueError("src_block_ids and dst_block_ids must be 1-D of equal length")
+    if validate and src.numel():
+        hs, hd = src.cpu(), dst.cpu()  # host ids as they are; device ids: one synchronising copy
+        if int(hs.min()) < 0 or int(hs.max()) >= num_blocks or int(hd.min()) < 0 or int(hd.max()) >= num_blocks:
+            raise IndexError(f"block id out of range [0, {num_blocks})")
+        d = set(hd.tolist())
+        if len(d) != hd.numel():
+            raise ValueError("destination block ids must be unique")
+        if d & set(hs.tolist()):
+            raise ValueError("a destination block is also a source block")
+    if src.numel() == 0:
+        return None, None
+    return (src.to(device, non_blocking=True).contiguous(), dst.to(device, non_blocking=True).contiguous())
 
 
 class _PagedKVCache:
@@ -113,26 +135,11 @@ class _PagedKVCache:
         as they are, device ids after one copy to the host (a synchronisation;
         ``validate=False`` skips it for ids the caller has already checked --
         the kernel then skips ids outside the pool)."""
-        src = torch.as_tensor(src_block_ids, dtype=torch.int64)
-        dst = torch.as_tensor(dst_block_ids, dtype=torch.int64)
-        if src.shape != dst.shape or src.dim() != 1:
-            raise ValueError("src_block_ids and dst_block_ids must be 1-D of equal length")
-        n = self.kv_cache.shape[2]
-        if validate and src.numel():
-            hs, hd = src.cpu(), dst.cpu()  # host ids as they are; device ids: one synchronising copy
-            if int(hs.min()) < 0 or int(hs.max()) >= n or int(hd.min()) < 0 or int(hd.max()) >= n:
-                raise IndexError(f"block id out of range [0, {n})")
-            d = set(hd.tolist())
-            if len(d) != hd.numel():
-                raise ValueError("destination block ids must be unique")
-            if d & set(hs.tolist()):
-                raise ValueError("a destination block is also a source block")
-        if src.numel() == 0:
-            return
-        dev = self.kv_cache.device
-        src = src.to(dev, non_blocking=True).contiguous()
-        dst = dst.to(dev, non_blocking=True).contiguous()
         kv = self.kv_cache
+        dev, n = kv.device, kv.shape[2]
+        src, dst = _checked_pairs(src_block_ids, dst_block_ids, n, validate, dev)
+        if src is None:
+            return
         es = kv.element_size()
         block_bytes = kv[0, 0, 0].numel() * es
         if _dense(kv[0, 0, 0]):
@@ -157,9 +164,10 @@ class _PagedKVCache:
 def hip_paged_attention_forward(module, query, key, value, attention_mask, scaling, **kwargs):
     """HF attention-interface function (serving_engine/model_runner.py:48-59):
     append this layer's K/V, then paged attention over the block pool.
-    query [1, Hq, S, D], key/value [1, Hkv, S, D]; kwargs cache, write_index,
-    paged_metadata.  Returns ([1, S, Hq, D], None)."""
-    cache: _PagedKVCache = kwargs["cache"]
+    query [1, Hq, S, D], key/value [1, Hkv, S, D]; kwargs cache (a _PagedKVCache
+    or a _PagedKVCache4Bit), write_index, paged_metadata.  Returns
+    ([1, S, Hq, D], None)."""
+    cache = kwargs["cache"]
     if type(cache) is _PagedKVCache:
         # Both launches from one native call (None: a call for the code below;
         # False: the attention is, its append is queued).
@@ -169,6 +177,12 @@ def hip_paged_attention_forward(module, query, key, value, attention_mask, scali
             _attention._WORKSPACES)
         if isinstance(o, torch.Tensor):
             return o, None
+    elif isinstance(cache, _PagedKVCache4Bit):
+        cache.write(key, value, module.layer_idx, kwargs["write_index"])
+        q = query.transpose(1, 2).squeeze(0)  # [S, Hq, D]
+        o, _ = paged_flash_attention_4bit(q, cache.blocks(module.layer_idx), kwargs["paged_metadata"], q.shape[1],
+                                          cache.num_kv_heads, scaling)
+        return o.unsqueeze(0), None
     else:
         o = None
     if o is None:
@@ -268,8 +282,10 @@ def step_inputs(scheduler_output, device="cuda", cache=None):
             raise ValueError("the step has copy-on-write block copies: pass the cache")
         src, dst = zip(*copies)
         cache.copy_blocks(list(src), list(dst))
-    meta = build_paged_batch_metadata(scheduler_output, device=device,
-                                      num_blocks=cache.kv_cache.shape[2] if cache is not None else None)
+    pool = None
+    if cache is not None:
+        pool = cache.num_blocks if isinstance(cache, _PagedKVCache4Bit) else cache.kv_cache.shape[2]
+    meta = build_paged_batch_metadata(scheduler_output, device=device, num_blocks=pool)
     return meta, meta.get("slot_mapping"), meta.get("positions")
 
 

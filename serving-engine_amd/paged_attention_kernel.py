@@ -392,3 +392,69 @@ def build_slot_mapping(metadata, block_size=BLOCK_SIZE, out=None):
         slots.data_ptr(), positions.data_ptr(), _lib.stream_handle(device))
     _lib.check(status, "kvhot_build_slot_mapping")
     return slots, positions
+
+
+def build_block_tables(block_table, prior_lens, q_lens, free_blocks, total_query, max_q_len, max_k_len=None,
+                       block_size=BLOCK_SIZE):
+    """A step's metadata built on the GPU from the lengths of its rows, for
+    steps whose lengths the host does not know (after drafted tokens were
+    accepted on the device, say): build_paged_batch_metadata without the host.
+
+    Row r has prior_lens[r] cached tokens, in the first ceil(prior_lens[r] /
+    block_size) blocks of block_table[r], and adds q_lens[r]; the blocks it
+    needs beyond those are the next ones of free_blocks [F], row by row, and are
+    entered into block_table, in place.  All int32 on one GPU; block_table
+    [R, MB], the lengths [R].  total_query: length of the slot mapping and the
+    positions, at least the sum of q_lens (the tokens beyond it get slot -1,
+    which an append skips, and position 0).  max_q_len and max_k_len (the
+    table's MB * block_size by default) bound the rows' lengths.
+
+    Returns the metadata dict of paged_flash_attention (and of
+    paged_flash_attention_4bit), without host copies, plus ``slot_mapping``,
+    ``positions`` and ``blocks_taken``: int32 [1], the blocks that the rows
+    need beyond those they hold.  Where that is above F, the missing ones are
+    entered as block 0 and their tokens' slots are -1; the caller has to look.
+    Repeating a call repeats its results.
+    """
+    device = block_table.device
+    if device.type != "cuda":
+        raise ValueError("block_table must be on a GPU")
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [rows, blocks], got {tuple(block_table.shape)}")
+    r, mb = block_table.shape
+    for name, t, n in (("block_table", block_table, r), ("prior_lens", prior_lens, r), ("q_lens", q_lens, r),
+                       ("free_blocks", free_blocks, None)):
+        _check_meta(name, t, device, n)
+        if name != "block_table" and t.dim() != 1:
+            raise ValueError(f"{name} must be 1-D, got {tuple(t.shape)}")
+    total, max_q = int(total_query), int(max_q_len)
+    if total < 0 or max_q < 0 or block_size <= 0:
+        raise ValueError("total_query, max_q_len and block_size must not be negative")
+    ints = torch.empty(2 * r + 1, dtype=torch.int32, device=device)
+    longs = torch.empty(2 * total, dtype=torch.int64, device=device)
+    meta = {
+        "q_lens": q_lens,
+        "k_lens": ints[:r],
+        "q_starts": ints[r:2 * r],
+        "q_pos_offsets": prior_lens,
+        "block_table": block_table,
+        "block_table_row_stride": mb,
+        "total_query": total,
+        "max_q_len": max_q,
+        "max_k_len": mb * block_size if max_k_len is None else int(max_k_len),
+        "slot_mapping": longs[:total],
+        "positions": longs[total:],
+        "blocks_taken": ints[2 * r:],
+    }
+    if r == 0:
+        longs[:total] = -1
+        longs[total:] = 0
+        ints.zero_()
+        return meta
+    with torch.cuda.device(device):
+        status = _lib.load().kvhot_build_block_tables(
+            block_table.data_ptr(), mb, prior_lens.data_ptr(), q_lens.data_ptr(), free_blocks.data_ptr(),
+            free_blocks.shape[0], r, total, max_q, block_size, meta["q_starts"].data_ptr(), meta["k_lens"].data_ptr(),
+            longs.data_ptr(), meta["positions"].data_ptr(), meta["blocks_taken"].data_ptr(), _lib.stream_handle(device))
+    _lib.check(status, "kvhot_build_block_tables")
+    return meta
