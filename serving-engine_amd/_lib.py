@@ -85,7 +85,7 @@ SIGNATURES = {
     ),
 }
 
-# The same for include/kvhot_layer.h.
+# The same for include/kvhot_layer.h, in its order (bind_layer's).
 LAYER_SIGNATURES = {
     "kvhot_build_block_tables": (
         _int,
@@ -157,6 +157,7 @@ def native():
                               "`python serving-engine_amd/build.py`") from e
         kvhot_torch.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "kvhot_paged_attention", "kvhot_paged_attention_workspace_bytes", "kvhot_reshape_and_cache")))
+        kvhot_torch.bind_layer(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in LAYER_SIGNATURES))
         _NATIVE = kvhot_torch
     return _NATIVE
 

@@ -1,6 +1,7 @@
 // The per-layer calls of an engine step, from torch tensors to libkvhot's
 // entry points without Python in between: paged_flash_attention, the append
-// (_PagedKVCache.write) and the two together (a model's layer).
+// (_PagedKVCache.write) and the two together (a model's layer); and the same for
+// the cache held in 4 bits, norm_rope and build_block_tables.
 //
 // Every function here answers the ordinary call only, after checking all that
 // the Python function of the same name checks, and returns None before it has
@@ -27,6 +28,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/kvhot.h"
+#include "../../include/kvhot_layer.h"
 
 namespace {
 
@@ -35,11 +37,17 @@ using at::Tensor;
 decltype(&kvhot_paged_attention) g_attention = nullptr;
 decltype(&kvhot_paged_attention_workspace_bytes) g_workspace_bytes = nullptr;
 decltype(&kvhot_reshape_and_cache) g_append = nullptr;
+decltype(&kvhot_build_block_tables) g_tables = nullptr;
+decltype(&kvhot_norm_rope) g_norm_rope = nullptr;
+decltype(&kvhot_reshape_and_cache_4bit) g_append4 = nullptr;
+decltype(&kvhot_read_cache_4bit) g_read4 = nullptr;
+decltype(&kvhot_paged_attention_4bit_workspace_bytes) g_workspace_bytes4 = nullptr;
+decltype(&kvhot_paged_attention_4bit) g_attention4 = nullptr;
 
 // Keys of the metadata dict and of its launch lists.
 struct Names {
   PyObject *q_lens, *k_lens, *q_starts, *q_pos_offsets, *block_table, *block_table_row_stride, *max_q_len, *max_k_len,
-      *host_q_lens, *schedules, *schedule_streams;
+      *host_q_lens, *schedules, *schedule_streams, *total_query, *slot_mapping, *positions, *blocks_taken;
 } g_names;
 
 // The plain torch.Tensor behind o, with memory on a GPU.  (Subclasses and
@@ -75,6 +83,21 @@ bool as_int(PyObject* o, int64_t& x) {
 bool meta_tensor(PyObject* meta, PyObject* name, c10::Device d, int64_t n, Tensor& t) {
   return gpu_tensor(PyDict_GetItemWithError(meta, name), t) && t.scalar_type() == at::kInt && t.device() == d &&
          t.is_contiguous() && t.dim() >= 1 && t.size(0) == n;
+}
+
+// The stream's workspace, made by the first call that needed it, if it holds
+// `need` bytes; none under capture (a graph's calls have workspaces of their
+// own).
+bool stream_workspace(PyObject* workspaces, c10::Device d, void* stream, int64_t need, Tensor& ws) {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) != hipSuccess) (void)hipGetLastError();
+  if (capture != hipStreamCaptureStatusNone) return false;
+  PyObject* key = Py_BuildValue("(iL)", static_cast<int>(d.index()),
+                                static_cast<long long>(reinterpret_cast<intptr_t>(stream)));
+  if (!key) return false;
+  PyObject* w = PyDict_GetItemWithError(workspaces, key);
+  Py_DECREF(key);
+  return gpu_tensor(w, ws) && ws.numel() >= need;
 }
 
 // One layer's append: K and V new rows [1, Hkv, S, D] into the pool.
@@ -188,20 +211,7 @@ struct Attention {
       need = g_workspace_bytes(rows, q.size(0), max_q, max_k, hq, hkv, dim, block_size, pt, dt);
       if (need < 0) return false;
     }
-    if (need > 0) {  // the stream's workspace, made by the first call that needs it
-      hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-      if (hipStreamIsCapturing(static_cast<hipStream_t>(stream), &capture) != hipSuccess)
-        (void)hipGetLastError();
-      if (capture != hipStreamCaptureStatusNone)
-        return false;  // a graph's calls have workspaces of their own
-      PyObject* key = Py_BuildValue("(iL)", static_cast<int>(d.index()),
-                                    static_cast<long long>(reinterpret_cast<intptr_t>(stream)));
-      if (!key) return false;
-      PyObject* w = PyDict_GetItemWithError(workspaces, key);
-      Py_DECREF(key);
-      if (!gpu_tensor(w, ws) || ws.numel() < need) return false;
-    }
-    return true;
+    return need == 0 || stream_workspace(workspaces, d, stream, need, ws);
   }
 
   int launch(const Tensor& o, const Tensor& l) const {
@@ -246,6 +256,14 @@ Tensor lse_of(const Tensor& q) {
   return at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat).requires_grad(false).memory_format(c10::nullopt));
 }
 
+PyObject* pair_of(const Tensor& x, const Tensor& y) {
+  PyObject* r = PyTuple_New(2);
+  if (!r) return nullptr;
+  PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(x));
+  PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(y));
+  return r;
+}
+
 // attention(q, k_cache, v_cache, metadata, hq, hkv, scale, causal, pt, flags, workspaces) -> (o, l) | None
 PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return or_none([&]() -> PyObject* {
@@ -271,11 +289,7 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!at_.check(a[3], a[6], pt, a[7] == Py_True, static_cast<int>(flags), a[10])) return nullptr;
     const Tensor o = at::empty_like(q, q.options().requires_grad(false)), l = lse_of(q);
     if (without_gil([&] { return at_.launch(o, l); }) != 0) return nullptr;
-    PyObject* r = PyTuple_New(2);
-    if (!r) return nullptr;
-    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(o));
-    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(l));
-    return r;
+    return pair_of(o, l);
   });
 }
 
@@ -329,6 +343,243 @@ PyObject* py_layer(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ------------------------------------------------------- include/kvhot_layer.h
+
+// Whether t's device is the current one (the Python functions switch to it).
+bool on_current_device(const Tensor& t) {
+  int now = -1;
+  return hipGetDevice(&now) == hipSuccess && now == t.get_device();
+}
+
+bool index_tensor(const Tensor& t, c10::Device d) {
+  return t.dim() == 1 && (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt) && t.is_contiguous() &&
+         t.device() == d;
+}
+
+bool is_long(const Tensor& t) { return t.scalar_type() == at::kLong; }
+
+// A layer of a cache held in 4 bits: records [N, S, Hkv, 17 D].
+struct Pool4Bit {
+  Tensor pool;  // [L, N, S, Hkv, 17 D]
+  int64_t layer, dim;
+
+  bool check(PyObject* pool_o, PyObject* dim_o, PyObject* layer_o) {
+    return gpu_tensor(pool_o, pool) && as_int(dim_o, dim) && as_int(layer_o, layer) && pool.dim() == 5 &&
+           pool.scalar_type() == at::kByte && layer >= 0 && layer < pool.size(0) && pool.size(4) == 17 * dim &&
+           pool.stride(4) == 1 && pool.stride(3) == 17 * dim && pool.stride(2) == pool.size(3) * 17 * dim &&
+           on_current_device(pool);
+  }
+  char* base() const { return static_cast<char*>(pool.data_ptr()) + layer * pool.stride(0); }
+  int64_t heads() const { return pool.size(3); }
+  int64_t block_size() const { return pool.size(2) * 16; }
+};
+
+// append4(pool, dim, dtype, key, value, layer, slots) -> True | None
+PyObject* py_append4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return or_none([&]() -> PyObject* {
+    Pool4Bit p;
+    Tensor key, value, slots;
+    int64_t dtype;
+    if (n != 7 || !g_append4 || !p.check(a[0], a[1], a[5]) || !as_int(a[2], dtype) || !gpu_tensor(a[3], key) ||
+        !gpu_tensor(a[4], value) || !gpu_tensor(a[6], slots))
+      return nullptr;
+    const c10::Device d = p.pool.device();
+    if (key.dim() != 4 || key.size(0) != 1 || value.sizes() != key.sizes() || key.size(1) != p.heads() ||
+        key.size(3) != p.dim || key.size(2) == 0 || dtype_code(key) != dtype || dtype_code(value) != dtype ||
+        key.device() != d || value.device() != d || !index_tensor(slots, d) || slots.size(0) != key.size(2))
+      return nullptr;
+    const int64_t ks[3] = {key.stride(2), key.stride(1), key.stride(3)};
+    const int64_t vs[3] = {value.stride(2), value.stride(1), value.stride(3)};
+    void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
+    const int status = without_gil([&] {
+      return g_append4(key.data_ptr(), ks, value.data_ptr(), vs, p.base(), p.pool.stride(1), slots.data_ptr(),
+                       is_long(slots), key.size(2), p.heads(), p.dim, p.block_size(), p.pool.size(1),
+                       static_cast<int>(dtype), stream);
+    });
+    if (status != 0) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// read4(pool, dim, dtype, layer, slots) -> (key, value) | None
+PyObject* py_read4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return or_none([&]() -> PyObject* {
+    Pool4Bit p;
+    Tensor slots;
+    int64_t dtype;
+    if (n != 5 || !g_read4 || !p.check(a[0], a[1], a[3]) || !as_int(a[2], dtype) || !gpu_tensor(a[4], slots) ||
+        !index_tensor(slots, p.pool.device()) || slots.size(0) == 0)
+      return nullptr;
+    const at::ScalarType type = dtype == KVHOT_F32 ? at::kFloat : dtype == KVHOT_F16 ? at::kHalf : at::kBFloat16;
+    const auto options = p.pool.options().dtype(type);
+    const Tensor key = at::empty({slots.size(0), p.heads(), p.dim}, options), value = at::empty(key.sizes(), options);
+    void* stream = c10::hip::getCurrentHIPStream(p.pool.get_device()).stream();
+    const int status = without_gil([&] {
+      return g_read4(p.base(), p.pool.stride(1), slots.data_ptr(), is_long(slots), slots.size(0), p.heads(), p.dim,
+                     p.block_size(), p.pool.size(1), key.data_ptr(), value.data_ptr(), static_cast<int>(dtype), stream);
+    });
+    if (status != 0) return nullptr;
+    return pair_of(key, value);
+  });
+}
+
+// attention4(q, blocks, metadata, hq, hkv, scale, causal, workspaces) -> (o, l) | None
+PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return or_none([&]() -> PyObject* {
+    Tensor q, kv, q_lens, k_lens, q_starts, q_offs, bt, ws;
+    int64_t hq, hkv, max_q, max_k, bt_stride;
+    if (n != 8 || !g_attention4 || !g_workspace_bytes4 || !gpu_tensor(a[0], q) || !gpu_tensor(a[1], kv) ||
+        !PyDict_CheckExact(a[2]) || !as_int(a[3], hq) || !as_int(a[4], hkv) || !PyFloat_Check(a[5]) || !PyBool_Check(a[6]) ||
+        !PyDict_CheckExact(a[7]))
+      return nullptr;
+    PyObject* meta = a[2];
+    const int dt = dtype_code(q);
+    const c10::Device d = q.device();
+    if (q.dim() != 3 || kv.dim() != 4 || kv.scalar_type() != at::kByte || kv.device() != d || dt < 0 || hkv <= 0 || hq <= 0 ||
+        hq % hkv != 0 || q.size(1) != hq || q.size(0) == 0 || kv.size(2) != hkv || kv.size(3) != 17 * q.size(2) ||
+        kv.stride(3) != 1 || kv.stride(2) != kv.size(3) || kv.stride(1) != hkv * kv.size(3) || !on_current_device(q))
+      return nullptr;
+    if (!gpu_tensor(PyDict_GetItemWithError(meta, g_names.q_lens), q_lens) || q_lens.dim() < 1) return nullptr;
+    const int64_t rows = q_lens.size(0);
+    if (rows == 0 || !meta_tensor(meta, g_names.q_lens, d, rows, q_lens) || !meta_tensor(meta, g_names.k_lens, d, rows, k_lens) ||
+        !meta_tensor(meta, g_names.q_starts, d, rows, q_starts) || !meta_tensor(meta, g_names.q_pos_offsets, d, rows, q_offs) ||
+        !meta_tensor(meta, g_names.block_table, d, rows, bt) ||
+        !as_int(PyDict_GetItemWithError(meta, g_names.block_table_row_stride), bt_stride) ||
+        !as_int(PyDict_GetItemWithError(meta, g_names.max_q_len), max_q) ||
+        !as_int(PyDict_GetItemWithError(meta, g_names.max_k_len), max_k))
+      return nullptr;
+    const int64_t need = g_workspace_bytes4(rows, q.size(0), max_q, max_k, hq, hkv, q.size(2), dt);
+    void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
+    if (need < 0 || (need > 0 && !stream_workspace(a[7], d, stream, need, ws))) return nullptr;
+    const Tensor o = at::empty_like(q, q.options().requires_grad(false)), l = lse_of(q);
+    const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)}, os[3] = {o.stride(0), o.stride(1), o.stride(2)};
+    const int64_t ls[2] = {l.stride(0), l.stride(1)};
+    const float scale = static_cast<float>(PyFloat_AS_DOUBLE(a[5]));
+    const int flags = a[6] == Py_True ? KVHOT_CAUSAL : 0;
+    const auto i32 = [](const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); };
+    const int status = without_gil([&] {
+      return g_attention4(q.data_ptr(), qs, kv.data_ptr(), kv.stride(0), o.data_ptr(), os, static_cast<float*>(l.data_ptr()),
+                          ls, i32(bt), bt_stride, i32(q_lens), i32(k_lens), i32(q_starts), i32(q_offs), rows, q.size(0),
+                          max_q, max_k, hq, hkv, q.size(2), kv.size(1) * 16, kv.size(0), scale, flags, dt,
+                          ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, stream);
+    });
+    if (status != 0) return nullptr;
+    return pair_of(o, l);
+  });
+}
+
+// norm_rope(q, k, positions, table, q_weight, k_weight, eps, interleaved) -> (q', k') | None
+PyObject* py_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return or_none([&]() -> PyObject* {
+    Tensor q, k, pos, table, w[2];
+    if (n != 8 || !g_norm_rope || !gpu_tensor(a[0], q) || !gpu_tensor(a[1], k) || !gpu_tensor(a[2], pos) ||
+        !gpu_tensor(a[3], table) || !PyFloat_Check(a[6]) || !PyBool_Check(a[7]))
+      return nullptr;
+    const int dt = dtype_code(q);
+    const c10::Device d = q.device();
+    if (q.dim() != 3 || k.dim() != 3 || dt < 0 || k.scalar_type() != q.scalar_type() || q.size(0) != k.size(0) ||
+        q.size(2) != k.size(2) || q.size(0) == 0 || k.device() != d || !index_tensor(pos, d) || pos.size(0) != q.size(0) ||
+        table.dim() != 2 || table.scalar_type() != at::kFloat || !table.is_contiguous() || table.device() != d ||
+        !on_current_device(q))
+      return nullptr;
+    int wdt = dt;
+    for (int i = 0; i < 2; ++i) {
+      if (a[4 + i] == Py_None) continue;
+      if (!gpu_tensor(a[4 + i], w[i]) || w[i].dim() != 1 || w[i].size(0) != q.size(2) || !w[i].is_contiguous() ||
+          w[i].device() != d || (w[i].scalar_type() != at::kFloat && w[i].scalar_type() != q.scalar_type()) ||
+          (i == 1 && w[0].defined() && w[0].scalar_type() != w[1].scalar_type()))
+        return nullptr;
+      wdt = dtype_code(w[i]);
+    }
+    const auto options = q.options().requires_grad(false);
+    const Tensor oq = at::empty(q.sizes(), options), ok = at::empty(k.sizes(), options);
+    const Tensor* t[4] = {&q, &k, &oq, &ok};
+    int64_t st[4][3];
+    for (int i = 0; i < 4; ++i)
+      for (int j = 0; j < 3; ++j) st[i][j] = t[i]->stride(j);
+    const auto weight = [&](int i) { return w[i].defined() ? w[i].data_ptr() : nullptr; };
+    const float eps = static_cast<float>(PyFloat_AS_DOUBLE(a[6]));
+    const int interleaved = a[7] == Py_True ? 1 : 0;
+    void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
+    const int status = without_gil([&] {
+      return g_norm_rope(q.data_ptr(), st[0], k.data_ptr(), st[1], oq.data_ptr(), st[2], ok.data_ptr(), st[3], weight(0),
+                         weight(1), wdt, eps, static_cast<const float*>(table.data_ptr()), table.size(0), table.size(1),
+                         interleaved, pos.data_ptr(), is_long(pos), q.size(0), q.size(1), k.size(1), q.size(2), dt, stream);
+    });
+    if (status != 0) return nullptr;
+    return pair_of(oq, ok);
+  });
+}
+
+// tables(block_table, prior_lens, q_lens, free_blocks, total, max_q, max_k, block_size) -> metadata dict | None
+PyObject* py_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return or_none([&]() -> PyObject* {
+    Tensor bt, prior, q_lens, free;
+    int64_t total, max_q, max_k, bs;
+    if (n != 8 || !g_tables || !gpu_tensor(a[0], bt) || !gpu_tensor(a[1], prior) || !gpu_tensor(a[2], q_lens) ||
+        !gpu_tensor(a[3], free) || !as_int(a[4], total) || !as_int(a[5], max_q) || !as_int(a[6], max_k) || !as_int(a[7], bs))
+      return nullptr;
+    const c10::Device d = bt.device();
+    const auto list = [&](const Tensor& t) {
+      return t.dim() == 1 && t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == d;
+    };
+    if (bt.dim() != 2 || bt.scalar_type() != at::kInt || !bt.is_contiguous() || !list(prior) || !list(q_lens) || !list(free) ||
+        prior.size(0) != bt.size(0) || q_lens.size(0) != bt.size(0) || bt.size(0) == 0 || total < 0 || max_q < 0 || bs <= 0 ||
+        !on_current_device(bt))
+      return nullptr;
+    const int64_t r = bt.size(0), mb = bt.size(1);
+    const Tensor ints = at::empty({2 * r + 1}, bt.options()), longs = at::empty({2 * total}, bt.options().dtype(at::kLong));
+    int32_t* const i = static_cast<int32_t*>(ints.data_ptr());
+    int64_t* const l = static_cast<int64_t*>(longs.data_ptr());
+    const auto i32 = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+    void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
+    const int status = without_gil([&] {
+      return g_tables(i32(bt), mb, i32(prior), i32(q_lens), i32(free), free.size(0), r, total, max_q, bs, i + r, i, l,
+                      l + total, i + 2 * r, stream);
+    });
+    if (status != 0) return nullptr;
+    PyObject* meta = PyDict_New();
+    if (!meta) return nullptr;
+    const auto put = [&](PyObject* name, PyObject* x) {  // takes x
+      const bool ok = x && PyDict_SetItem(meta, name, x) == 0;
+      Py_XDECREF(x);
+      return ok;
+    };
+    bool ok = true;
+    try {
+      ok = put(g_names.q_lens, Py_NewRef(a[2])) && put(g_names.k_lens, THPVariable_Wrap(ints.narrow(0, 0, r))) &&
+           put(g_names.q_starts, THPVariable_Wrap(ints.narrow(0, r, r))) && put(g_names.q_pos_offsets, Py_NewRef(a[1])) &&
+           put(g_names.block_table, Py_NewRef(a[0])) && put(g_names.block_table_row_stride, PyLong_FromLongLong(mb)) &&
+           put(g_names.total_query, PyLong_FromLongLong(total)) && put(g_names.max_q_len, PyLong_FromLongLong(max_q)) &&
+           put(g_names.max_k_len, PyLong_FromLongLong(max_k)) &&
+           put(g_names.slot_mapping, THPVariable_Wrap(longs.narrow(0, 0, total))) &&
+           put(g_names.positions, THPVariable_Wrap(longs.narrow(0, total, total))) &&
+           put(g_names.blocks_taken, THPVariable_Wrap(ints.narrow(0, 2 * r, 1)));
+    } catch (...) {
+      ok = false;
+    }
+    if (!ok) {
+      Py_DECREF(meta);
+      return nullptr;
+    }
+    return meta;
+  });
+}
+
+// bind_layer(addresses of kvhot_layer.h's entry points, in its order)
+PyObject* py_bind_layer(PyObject*, PyObject* args) {
+  unsigned long long f[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", f, f + 1, f + 2, f + 3, f + 4, f + 5)) return nullptr;
+  const auto at = [&](int i) { return static_cast<uintptr_t>(f[i]); };
+  g_tables = reinterpret_cast<decltype(g_tables)>(at(0));
+  g_norm_rope = reinterpret_cast<decltype(g_norm_rope)>(at(1));
+  g_append4 = reinterpret_cast<decltype(g_append4)>(at(2));
+  g_read4 = reinterpret_cast<decltype(g_read4)>(at(3));
+  g_workspace_bytes4 = reinterpret_cast<decltype(g_workspace_bytes4)>(at(4));
+  g_attention4 = reinterpret_cast<decltype(g_attention4)>(at(5));
+  Py_RETURN_NONE;
+}
+
 // bind(attention, workspace_bytes, append): addresses of libkvhot's entry points.
 PyObject* py_bind(PyObject*, PyObject* args) {
   unsigned long long at, ws, ap;
@@ -344,6 +595,12 @@ PyMethodDef kMethods[] = {
     {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_append)), METH_FASTCALL, nullptr},
     {"layer", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_layer)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_VARARGS, nullptr},
+    {"append4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_append4)), METH_FASTCALL, nullptr},
+    {"read4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_read4)), METH_FASTCALL, nullptr},
+    {"attention4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention4)), METH_FASTCALL, nullptr},
+    {"norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_norm_rope)), METH_FASTCALL, nullptr},
+    {"tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_tables)), METH_FASTCALL, nullptr},
+    {"bind_layer", py_bind_layer, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "kvhot_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
@@ -363,5 +620,9 @@ PyMODINIT_FUNC PyInit_kvhot_torch(void) {
   g.host_q_lens = PyUnicode_InternFromString("host_q_lens");
   g.schedules = PyUnicode_InternFromString("_schedules");
   g.schedule_streams = PyUnicode_InternFromString("_schedule_streams");
+  g.total_query = PyUnicode_InternFromString("total_query");
+  g.slot_mapping = PyUnicode_InternFromString("slot_mapping");
+  g.positions = PyUnicode_InternFromString("positions");
+  g.blocks_taken = PyUnicode_InternFromString("blocks_taken");
   return PyModule_Create(&kModule);
 }

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .block import BLOCK_SIZE
-from .paged_attention_kernel import _check_meta, _host_max, _workspace
+from .paged_attention_kernel import _WORKSPACES, _check_meta, _host_max, _workspace
 
 HEAD_DIMS_4BIT = (64, 96, 128, 256)
 RECORD_TOKENS = 16  # tokens of a record; a block holds block_size / 16 of them a kv head
@@ -65,7 +65,7 @@ class _PagedKVCache4Bit:
         _check_blocks(kv_cache, 5)
         if kv_cache.shape[4] != record_bytes_4bit(head_dim):
             raise ValueError(f"records of {kv_cache.shape[4]} bytes do not hold head_dim {head_dim}")
-        _lib.dtype_code(dtype)
+        self._code = _lib.dtype_code(dtype)
         self.kv_cache = kv_cache
         self.num_kv_heads = kv_cache.shape[3]
         self.head_dim = head_dim
@@ -100,7 +100,12 @@ class _PagedKVCache4Bit:
         the smallest power of two s with max|x| <= 7 s, held to [2^-125, 2^125]
         ([2^-23, 2^13] in fp16); codes are the nearest, ties to the even one.
         Elements that share a scale with an infinity or a NaN become NaN.
-        Slots outside the pool are skipped; those inside must be distinct."""
+        Slots outside the pool are skipped; those inside must be distinct.
+        (The ordinary call runs in kvhot_torch, as those of read and
+        paged_flash_attention_4bit do; the rest here.)"""
+        if _lib.native().append4(self.kv_cache, self.head_dim, self._code, key_states, value_states, layer_idx,
+                                 write_index):
+            return
         shape = key_states.shape
         if len(shape) != 4 or shape[0] != 1 or value_states.shape != shape:
             raise ValueError(f"key {tuple(key_states.shape)} / value {tuple(value_states.shape)} must be [1, Hkv, S, D]")
@@ -129,6 +134,9 @@ class _PagedKVCache4Bit:
         """What the cache holds at slots read_index: K and V, each a dense
         [len(read_index), Hkv, D] of the cache's dtype (zeros for a slot outside
         the pool)."""
+        out = _lib.native().read4(self.kv_cache, self.head_dim, self._code, layer_idx, read_index)
+        if out is not None:
+            return out
         read_index = self._index("read_index", read_index)
         base = self._layer(layer_idx)
         kv, n = self.kv_cache, read_index.shape[0]
@@ -184,6 +192,9 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     cache reaches the queries that see it and no other; in fp16, cached values beyond
     its range (of a pool written from another dtype) are infinite.
     """
+    out = _lib.native().attention4(q, kv_blocks, metadata, num_q_heads, num_kv_heads, scale, bool(is_causal), _WORKSPACES)
+    if out is not None:
+        return out
     if q.dim() != 3:
         raise ValueError("expected q [T, Hq, D]")
     _check_blocks(kv_blocks, 4)

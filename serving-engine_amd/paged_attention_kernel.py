@@ -414,8 +414,14 @@ def build_block_tables(block_table, prior_lens, q_lens, free_blocks, total_query
     ``positions`` and ``blocks_taken``: int32 [1], the blocks that the rows
     need beyond those they hold.  Where that is above F, the missing ones are
     entered as block 0 and their tokens' slots are -1; the caller has to look.
-    Repeating a call repeats its results.
+    Repeating a call repeats its results.  (The ordinary call runs in
+    kvhot_torch, the rest here.)
     """
+    if max_k_len is None and block_table.dim() == 2:
+        max_k_len = block_table.shape[1] * block_size
+    meta = _lib.native().tables(block_table, prior_lens, q_lens, free_blocks, total_query, max_q_len, max_k_len, block_size)
+    if meta is not None:
+        return meta
     device = block_table.device
     if device.type != "cuda":
         raise ValueError("block_table must be on a GPU")
@@ -441,7 +447,7 @@ def build_block_tables(block_table, prior_lens, q_lens, free_blocks, total_query
         "block_table_row_stride": mb,
         "total_query": total,
         "max_q_len": max_q,
-        "max_k_len": mb * block_size if max_k_len is None else int(max_k_len),
+        "max_k_len": int(max_k_len),
         "slot_mapping": longs[:total],
         "positions": longs[total:],
         "blocks_taken": ints[2 * r:],

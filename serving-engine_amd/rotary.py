@@ -38,8 +38,13 @@ def norm_rope(q, k, positions, table, q_weight=None, k_weight=None, eps=1e-6, in
     outside the table makes its token's rows NaN.
 
     Returns (q', k'): new contiguous tensors, or ``out``, a pair which may be
-    (q, k) itself but must not overlap them otherwise.
+    (q, k) itself but must not overlap them otherwise.  (The ordinary call runs
+    in kvhot_torch, the rest here.)
     """
+    if out is None:
+        done = _lib.native().norm_rope(q, k, positions, table, q_weight, k_weight, eps, bool(interleaved))
+        if done is not None:
+            return done
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"q {tuple(q.shape)} / k {tuple(k.shape)} must be [T, Hq, D] and [T, Hkv, D]")
     t, hq, d = q.shape
