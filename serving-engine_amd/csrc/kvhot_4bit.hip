@@ -31,6 +31,10 @@
 #include <initializer_list>
 #include <type_traits>
 
+#ifndef KVHOT_W4
+#define KVHOT_W4 3
+#endif
+
 namespace kvhot {
 
 // Smallest and largest scale byte by dtype: half the smallest scale and six
@@ -224,10 +228,11 @@ struct Attn4Args {
   const int32_t *q_lens, *k_lens, *q_starts, *q_offs;
   int64_t total_query;
   int32_t num_rows, hq, hkv, group, block_size, num_blocks, causal;
-  float scale;  // times log2(e)
+  float scale;     // |scale| * log2(e)
+  int32_t negate;  // the scale is negative: Q's sign is turned
   int32_t q_vec, o_vec;
   // the padded grid
-  int32_t q_blocks, parts, part_steps, max_k;
+  int32_t q_blocks, parts, part_steps, max_k, spb;
   float* ws_o;
   float* ws_lse;
 };
@@ -276,14 +281,17 @@ __device__ inline bool block_of(const Attn4Args& a, int row, int head, int qb, B
   return true;
 }
 
-// Bytes of a step that a lane holds.
+// Codes and scales of a step that a lane holds.
 template <int D>
-struct Step4 {
+struct Keys4 {
   static constexpr int NJ = D / 32;
-  uint32_t k[4][NJ];   // codes of token 4 t + (lane & 3), elements 8 * NJ * (lane / 16) on
-  uint32_t ks[2];      // their scales, one byte for each t: of the first and the last element's group
-  u32x4 v[NJ];         // codes of the 16 tokens of record lane / 16, pairs pair_of(lane & 15, c)
-  u32x4 vs[D == 96 ? 3 : 1];  // their scales
+  uint32_t code[4][NJ];  // token 4 t + (lane & 3) of record (lane & 15) / 4, elements 8 * NJ * (lane / 16) on
+  uint32_t scale[2];     // one byte for each t: of the first and the last element's group
+};
+template <int D>
+struct Values4 {
+  u32x4 code[D / 32];             // the 16 tokens of record lane / 16, pairs pair_of(lane & 15, c)
+  u32x4 scale[D == 96 ? 3 : 1];   // theirs
 };
 
 // Pair of elements c of A row i of O^T's tiles.  At head_dim 96 an i has one
@@ -291,44 +299,60 @@ struct Step4 {
 template <int D>
 __device__ constexpr int pair_of(int i, int c) { return D == 96 ? i + 16 * c : (D / 32) * i + c; }
 
-template <int D>
-__device__ inline void load_step(const Attn4Args& a, const Block4& b, int step, int lane, Step4<D>& s) {
-  constexpr int NJ = Step4<D>::NJ;
-  constexpr int REC = 17 * D;
-  const int i = lane & 15, g = lane >> 4;
-  const int spb = a.block_size >> 4;
+// Where a lane's records of a step lie: the block ids come first, so that they
+// can be asked for a step ahead.
+struct Where4 {
+  int32_t k_id, v_id, k_in, v_in;  // block, record in it
+};
+
+__device__ inline Where4 where(const Attn4Args& a, const Block4& b, int step, int lane) {
   const int last = (b.limit + 15) / 16 - 1;
+  const int ks = imin(step * 4 + ((lane & 15) >> 2), last), vs = imin(step * 4 + (lane >> 4), last);
   const int32_t* bt = a.bt + static_cast<int64_t>(b.row) * a.bt_stride;
-  const auto rec = [&](int slice) {
-    slice = imin(slice, last);
-    const int blk = slice / spb;
-    const int id = imin(imax(bt[blk], 0), a.num_blocks - 1);
-    return a.cache + id * a.block_stride + (static_cast<int64_t>(slice - blk * spb) * a.hkv + b.head) * REC;
-  };
-  const char* kr = rec(step * 4 + (i >> 2));
-  const char* vr = rec(step * 4 + g);
+  if (a.spb == 1) return Where4{bt[ks], bt[vs], 0, 0};
+  const int kb = ks / a.spb, vb = vs / a.spb;
+  return Where4{bt[kb], bt[vb], ks - kb * a.spb, vs - vb * a.spb};
+}
+
+template <int D>
+__device__ inline const char* record_at(const Attn4Args& a, const Block4& b, int id, int in) {
+  id = imin(imax(id, 0), a.num_blocks - 1);
+  return a.cache + id * a.block_stride + (static_cast<int64_t>(in) * a.hkv + b.head) * (17 * D);
+}
+
+template <int D>
+__device__ inline void load_keys(const Attn4Args& a, const Block4& b, const Where4& w, int lane, Keys4<D>& s) {
+  constexpr int NJ = D / 32;
+  const int i = lane & 15, g = lane >> 4;
+  const char* kr = record_at<D>(a, b, w.k_id, w.k_in);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const char* p = kr + (4 * t + (i & 3)) * (D / 2) + g * (4 * NJ);
     if constexpr (NJ == 2) {
-      *reinterpret_cast<u32x2*>(s.k[t]) = *reinterpret_cast<const u32x2*>(p);
+      *reinterpret_cast<u32x2*>(s.code[t]) = *reinterpret_cast<const u32x2*>(p);
     } else if constexpr (NJ == 3) {
 #pragma unroll
-      for (int j = 0; j < 3; ++j) s.k[t][j] = reinterpret_cast<const uint32_t*>(p)[j];
+      for (int j = 0; j < 3; ++j) s.code[t][j] = reinterpret_cast<const uint32_t*>(p)[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < NJ; j += 4) *reinterpret_cast<u32x4*>(s.k[t] + j) = *reinterpret_cast<const u32x4*>(p + 4 * j);
+      for (int j = 0; j < NJ; j += 4) *reinterpret_cast<u32x4*>(s.code[t] + j) = *reinterpret_cast<const u32x4*>(p + 4 * j);
     }
   }
   const int g0 = (g * NJ) >> 2, g1 = (g * NJ + NJ - 1) >> 2;
-  s.ks[0] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g0 * 16 + (i & 3) * 4);
-  s.ks[1] = s.ks[0];
-  if constexpr (NJ == 3 || NJ == 8) s.ks[1] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g1 * 16 + (i & 3) * 4);
+  s.scale[0] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g0 * 16 + (i & 3) * 4);
+  s.scale[1] = s.scale[0];
+  if constexpr (NJ == 3 || NJ == 8) s.scale[1] = *reinterpret_cast<const uint32_t*>(kr + 16 * D + g1 * 16 + (i & 3) * 4);
+}
+
+template <int D>
+__device__ inline void load_values(const Attn4Args& a, const Block4& b, const Where4& w, int lane, Values4<D>& s) {
+  const int i = lane & 15;
+  const char* vr = record_at<D>(a, b, w.v_id, w.v_in);
 #pragma unroll
-  for (int c = 0; c < NJ; ++c) s.v[c] = *reinterpret_cast<const u32x4*>(vr + 8 * D + pair_of<D>(i, c) * 16);
+  for (int c = 0; c < D / 32; ++c) s.code[c] = *reinterpret_cast<const u32x4*>(vr + 8 * D + pair_of<D>(i, c) * 16);
 #pragma unroll
   for (int c = 0; c < (D == 96 ? 3 : 1); ++c)
-    s.vs[c] = *reinterpret_cast<const u32x4*>(vr + 16 * D + D / 2 + (pair_of<D>(i, c) >> 4) * 16);
+    s.scale[c] = *reinterpret_cast<const u32x4*>(vr + 16 * D + D / 2 + (pair_of<D>(i, c) >> 4) * 16);
 }
 
 // Running state of a wave: O^T tiles (tile 2 c + e holds element e of pair c),
@@ -358,15 +382,14 @@ __device__ inline void split_pair(float a, float b, uint32_t (&p)[NP]) {
   }
 }
 
-// Attends one step.  Q^T is q[tile][part][j]: element 8 (NJ * (lane / 16) + j) on
-// of m-row lane & 15.  MASKED: some m-row does not see all 64 keys.
-template <class M, int NP, int D, int MT, bool MASKED>
-__device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D / 32], const int (&sees)[MT], int base,
-                                   int limit, float scale, int lane, State4<D, MT>& st) {
+// S^T of a step: row 4 g + r of tile t is token 4 t + r of record g.  Q^T is
+// q[tile][part][j]: element 8 (NJ * (lane / 16) + j) on of m-row lane & 15.
+// (The barriers here and below keep the scheduler from converting everything
+// first, for which there are no registers.)
+template <class M, int NP, int D, int MT>
+__device__ inline void scores(const Keys4<D>& s, const u32x4 (&q)[MT][NP][D / 32], int lane, f32x4 (&sc)[MT][4]) {
   constexpr int NJ = D / 32;
   const int g = lane >> 4;
-  // S^T: row 4 g + r of tile t is token 4 t + r of record g.
-  f32x4 sc[MT][4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -374,17 +397,24 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const bool second = NJ == 8 ? j >= 4 : NJ == 3 ? ((g * 3 + j) >> 2) != ((g * 3) >> 2) : false;
-      const uint32_t sw = second ? s.ks[1] : s.ks[0];
-      const u32x4 k = codes8<M>(s.k[t][j], scale_of((sw >> (8 * t)) & 255));
+      const uint32_t sw = second ? s.scale[1] : s.scale[0];
+      const u32x4 k = codes8<M>(s.code[t][j], scale_of((sw >> (8 * t)) & 255));
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = NP - 1; n >= 0; --n) sc[m][t] = M::mfma(k, q[m][n][j], sc[m][t]);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
-  // Probabilities: lane (n, g) holds m-row n's for the 16 tokens of record g, the
-  // B operand of O^T's two products of 32 tokens.
-  u32x4 p[MT][NP][2];
+}
+
+// Probabilities from scores: lane (n, g) holds m-row n's for the 16 tokens of
+// record g, the B operand of O^T's two products of 32 tokens.  MASKED: some m-row
+// does not see all 64 keys.
+template <class M, int NP, int D, int MT, bool MASKED>
+__device__ inline void probabilities(f32x4 (&sc)[MT][4], const int (&sees)[MT], int base, float scale, int lane,
+                                     State4<D, MT>& st, u32x4 (&p)[MT][NP][2]) {
+  const int g = lane >> 4;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     float top = -INFINITY;
@@ -392,16 +422,14 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = sc[m][t][r] * scale;
-        if (MASKED && base + 16 * g + 4 * t + r >= sees[m]) x = -INFINITY;
-        sc[m][t][r] = x;
-        top = fmaxf(top, x);
+        if (MASKED && base + 16 * g + 4 * t + r >= sees[m]) sc[m][t][r] = -INFINITY;
+        top = fmaxf(top, sc[m][t][r]);
       }
-    if (__any(top > st.above[m])) {
+    if (__any(top * scale > st.above[m])) {
       top = fmaxf(top, __shfl_xor(top, 16, kWave));
       top = fmaxf(top, __shfl_xor(top, 32, kWave));
-      if (top > st.above[m]) {
-        const float ref = top - kBelow;
+      if (top * scale > st.above[m]) {
+        const float ref = top * scale - kBelow;
         const float f = st.above[m] == -INFINITY ? 0.0f : F32::exp2(st.ref[m] - ref);
         st.ref[m] = ref;
         st.above[m] = ref + kRoom;
@@ -416,7 +444,11 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const float x = BF16::exp2(sc[m][t][r] - st.ref[m]), y = BF16::exp2(sc[m][t][r + 1] - st.ref[m]);
+        float x = BF16::exp2(fmaf(sc[m][t][r], scale, -st.ref[m])), y = BF16::exp2(fmaf(sc[m][t][r + 1], scale, -st.ref[m]));
+        if (MASKED) {  // (a scale of 0 would make NaN of them)
+          if (base + 16 * g + 4 * t + r >= sees[m]) x = 0;
+          if (base + 16 * g + 4 * t + r + 1 >= sees[m]) y = 0;
+        }
         st.sum[m] += x + y;
         uint32_t w[NP];
         split_pair<M, NP>(x, y, w);
@@ -424,17 +456,24 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
         for (int n = 0; n < NP; ++n) p[m][n][t >> 1][(t & 1) * 2 + (r >> 1)] = w[n];
       }
   }
+}
+
+// O^T += V^T P^T.
+template <class M, int NP, int D, int MT, bool MASKED>
+__device__ inline void weigh(const Values4<D>& s, const u32x4 (&p)[MT][NP][2], const int (&sees)[MT], int base, int limit,
+                             int lane, State4<D, MT>& st) {
+  constexpr int NJ = D / 32, NS = D == 96 ? 3 : 1;
+  const int g = lane >> 4;
   // V's scales: one float a token.  In a masked step a NaN may belong to a key
   // that some m-row does not see, whose probability of 0 it would turn into NaN
   // too: it is taken out here and put into the m-rows that see it below.  What
   // lies behind the last key that any of them sees may be anything: its scales
   // are 1.
-  constexpr int NS = D == 96 ? 3 : 1;
   u32x4 vs[NS];
   uint32_t bad[NS];
 #pragma unroll
   for (int c = 0; c < NS; ++c) {
-    vs[c] = s.vs[c];
+    vs[c] = s.scale[c];
     bad[c] = 0;
     if (MASKED) {
 #pragma unroll
@@ -447,15 +486,21 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
     }
   }
 #pragma unroll
-  for (int c = 0; c < NJ; ++c) {
+  for (int u = 0; u < 2; ++u) {
+    float f[NS][8];  // of tokens 8 u .. 8 u + 7
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int c = 0; c < NS; ++c)
+#pragma unroll
+      for (int t = 0; t < 8; ++t) f[c][t] = scale_of((vs[c][2 * u + (t >> 2)] >> (8 * (t & 3))) & 255);
+#pragma unroll
+    for (int c = 0; c < NJ; ++c) {
       u32x4 lo, hi;  // elements 2 pair, 2 pair + 1 of tokens 8 u .. 8 u + 7
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const uint32_t code = s.v[c][2 * u + w], sb = vs[NS == 3 ? c : 0][2 * u + w];
-        const uint32_t a0 = pair16<M, 0>(code, scale_of(sb & 255)), a1 = pair16<M, 1>(code, scale_of((sb >> 8) & 255)),
-                       a2 = pair16<M, 2>(code, scale_of((sb >> 16) & 255)), a3 = pair16<M, 3>(code, scale_of(sb >> 24));
+        const uint32_t code = s.code[c][2 * u + w];
+        const float* x = f[NS == 3 ? c : 0] + 4 * w;
+        const uint32_t a0 = pair16<M, 0>(code, x[0]), a1 = pair16<M, 1>(code, x[1]), a2 = pair16<M, 2>(code, x[2]),
+                       a3 = pair16<M, 3>(code, x[3]);
         lo[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x05040100);
         lo[2 * w + 1] = __builtin_amdgcn_perm(a3, a2, 0x05040100);
         hi[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x07060302);
@@ -468,6 +513,7 @@ __device__ inline void attend_step(const Step4<D>& s, const u32x4 (&q)[MT][NP][D
           st.o[m][2 * c] = M::mfma(lo, p[m][n][u], st.o[m][2 * c]);
           st.o[m][2 * c + 1] = M::mfma(hi, p[m][n][u], st.o[m][2 * c + 1]);
         }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   if constexpr (MASKED) {
@@ -552,8 +598,11 @@ __device__ inline void park(const State4<D, MT>& a, float* lds, int lane) {
 template <int D, int MT>
 constexpr int parked() { return MT * (D / 16 * 4 + 3) * kWave; }
 
+// Waves a SIMD that the registers of an instantiation are for.
+constexpr int waves_per_simd(int np, int d, int mt) { return np == 3 ? (d == 256 ? 1 : 2) : d == 256 || mt == 2 ? 2 : KVHOT_W4; }
+
 template <class IO, class M, int NP, int D, int MT>
-__global__ void __launch_bounds__(64 * kWaves4)
+__global__ void __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NP, D, MT))))
 attn_4bit_kernel(Attn4Args a) {
   constexpr int NJ = D / 32, ROWS = 16 * MT;
   __shared__ float lds[kWaves4 / 2 * parked<D, MT>()];
@@ -593,6 +642,10 @@ attn_4bit_kernel(Attn4Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0;
       }
+      if (a.negate) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = -x[i];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         uint32_t w[NP];
@@ -611,19 +664,33 @@ attn_4bit_kernel(Attn4Args a) {
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) st.o[m][c] = f32x4{0, 0, 0, 0};
   }
-  if (step0 + wave < step1) {
-    Step4<D> cur;
-    load_step<D>(a, b, step0 + wave, lane, cur);
-    for (int s = step0 + wave; s < step1; s += kWaves4) {
-      Step4<D> next;
-      const bool more = s + kWaves4 < step1;
-      if (more) load_step<D>(a, b, s + kWaves4, lane, next);
-      if (s * kStep + kStep <= b.least)
-        attend_step<M, NP, D, MT, false>(cur, q, lim, s * kStep, b.limit, a.scale, lane, st);
-      else
-        attend_step<M, NP, D, MT, true>(cur, q, lim, s * kStep, b.limit, a.scale, lane, st);
-      if (more) cur = next;
-    }
+  // A step's keys are loaded while the step before is weighed, its values while
+  // its scores are computed; block ids two steps ahead.
+  int s = step0 + wave;
+  if (s < step1) {
+    Keys4<D> keys;
+    Values4<D> values;
+    Where4 w = where(a, b, s, lane);
+    load_keys<D>(a, b, w, lane, keys);
+    load_values<D>(a, b, w, lane, values);
+    w = where(a, b, imin(s + kWaves4, step1 - 1), lane);
+    const auto step = [&](auto masked) {
+      constexpr bool MASKED = decltype(masked)::value;
+      f32x4 sc[MT][4];
+      scores<M, NP, D, MT>(keys, q, lane, sc);
+      load_keys<D>(a, b, w, lane, keys);
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 p[MT][NP][2];
+      probabilities<M, NP, D, MT, MASKED>(sc, lim, s * kStep, a.scale, lane, st, p);
+      __builtin_amdgcn_sched_barrier(0);
+      weigh<M, NP, D, MT, MASKED>(values, p, lim, s * kStep, b.limit, lane, st);
+      load_values<D>(a, b, w, lane, values);
+      w = where(a, b, imin(s + 2 * kWaves4, step1 - 1), lane);
+      s += kWaves4;
+    };
+    const int full = imin(step1, b.least / kStep);  // steps that every m-row sees whole
+    while (s < full) step(std::false_type());
+    while (s < step1) step(std::true_type());
   }
   // The waves' states, joined in LDS: 2 and 3 into 0 and 1, then 1 into 0.
   if (wave >= 2) park<D, MT>(st, lds + (wave - 2) * parked<D, MT>(), lane);
@@ -954,13 +1021,15 @@ extern "C" int kvhot_paged_attention_4bit(
   a.block_size = static_cast<int32_t>(block_size);
   a.num_blocks = static_cast<int32_t>(num_blocks);
   a.causal = attn_flags & KVHOT_CAUSAL;
-  a.scale = scale * kLog2e;
+  a.scale = std::fabs(scale) * kLog2e;
+  a.negate = scale < 0;
   a.q_vec = aligned(q, es, 16, {q_strides[0], q_strides[1]});
   a.o_vec = aligned(out, es, 16, {out_strides[0], out_strides[1]});
   a.q_blocks = sp.q_blocks;
   a.parts = sp.parts;
   a.part_steps = sp.part_steps;
   a.max_k = static_cast<int32_t>(max_k_len);
+  a.spb = a.block_size / 16;
   a.ws_o = static_cast<float*>(workspace);
   a.ws_lse = a.ws_o ? a.ws_o + num_rows * sp.q_blocks * sp.parts * num_kv_heads * 16 * sp.mt * head_dim : nullptr;
   const hipStream_t s = static_cast<hipStream_t>(stream);
