@@ -93,15 +93,15 @@ __device__ inline void load8(const typename T::storage* p, bool vec, float (&x)[
   }
 }
 
-// The group's scale byte from a lane's share of it: four neighbouring lanes
-// hold 8 of its 32 values each.
+// The group's scale byte from a lane's share of it: lanes 16 apart hold 8 of its
+// 32 values each.
 __device__ inline uint32_t scale_byte(const float (&x)[8], uint32_t lo, uint32_t hi) {
   // As integers the magnitudes order like the floats, infinities and NaN on top.
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1, kWave)));
-  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2, kWave)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, kWave)));
+  top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, kWave)));
   if (top >= 0x7f800000u) return 255;
   const int e = static_cast<int>(top >> 23) + ((top & 0x7fffffu) > 0x600000u ? 1 : 0) - 2;
   return static_cast<uint32_t>(min(max(e, static_cast<int>(lo)), static_cast<int>(hi)));
@@ -120,37 +120,69 @@ __device__ inline uint32_t quantise8(const float (&x)[8], uint32_t byte) {
 
 // ------------------------------------------------------------------ append --
 
-// A lane quantises 8 elements of one (token, head) row of K or V.
-template <class T, typename SlotT>
+// A wave has 16 tokens of one head of K or V, GW groups of 32 elements in turn: lane
+// l has elements 8 (l / 16) on of token l % 16.  The 16 tokens of a prompt then lie
+// in the same lines of V, whose bytes of one pair are 16 tokens apart: with a
+// token's row in neighbouring lanes instead, 4152 tokens took 21 us.
+struct Unit4 {
+  int64_t t;  // the lane's token
+  int32_t head, group;
+  bool value, there;
+};
+
+template <int GW>
+__device__ inline Unit4 unit_of(int64_t tokens, int32_t heads, int32_t groups, int64_t units) {
+  Unit4 u;
+  int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  u.there = w < units;
+  const int32_t sets = groups / GW;
+  u.group = static_cast<int32_t>(w % sets) * GW;
+  w /= sets;
+  u.value = w & 1;
+  w >>= 1;
+  u.head = static_cast<int32_t>(w % heads);
+  u.t = w / heads * 16 + (threadIdx.x & 15);
+  u.there = u.there && u.t < tokens;
+  return u;
+}
+
+template <class T, typename SlotT, int GW>
 __global__ void __launch_bounds__(256)
 append_4bit_kernel(const typename T::storage* __restrict__ key, const typename T::storage* __restrict__ value,
-                   Pool4 pool, const SlotT* __restrict__ slots, int64_t per_kv, int32_t lanes_per_row, int64_t k_st,
-                   int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec, int v_vec, uint32_t lo, uint32_t hi) {
-  // (Whole quads are in or out: rows are a multiple of 4 lanes.)
-  int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (idx >= 2 * per_kv) return;
-  const bool is_v = idx >= per_kv;
-  if (is_v) idx -= per_kv;
-  const int64_t row = idx / lanes_per_row;
-  const int l = static_cast<int>(idx - row * lanes_per_row);
-  const int64_t t = row / pool.heads;
-  const int h = static_cast<int>(row - t * pool.heads);
-  const int d = lanes_per_row * 8;
-  int tok;
-  char* rec = record_of(pool, static_cast<int64_t>(slots[t]), h, tok);
-  float x[8];
-  load8<T>((is_v ? value + t * v_st + h * v_sh : key + t * k_st + h * k_sh) + l * 8, is_v ? v_vec : k_vec, x);
-  const uint32_t byte = scale_byte(x, lo, hi);
-  const uint32_t w = quantise8(x, byte);
-  if (!rec) return;
-  if (!is_v) {
-    *reinterpret_cast<uint32_t*>(rec + tok * (d / 2) + l * 4) = w;
-    if ((l & 3) == 0) rec[16 * d + (l >> 2) * 16 + (tok & 3) * 4 + (tok >> 2)] = static_cast<char>(byte);
-  } else {
-    char* v = rec + 8 * d + l * 64 + tok;
+                   Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int32_t groups, int64_t units,
+                   int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int k_vec, int v_vec, uint32_t lo,
+                   uint32_t hi) {
+  const Unit4 u = unit_of<GW>(tokens, pool.heads, groups, units);
+  const int l = (threadIdx.x & 63) >> 4, d = groups * 32;
+  float x[GW][8];
+  int tok = 0;
+  char* rec = nullptr;
+  if (u.there) {
+    rec = record_of(pool, static_cast<int64_t>(slots[u.t]), u.head, tok);
+    const typename T::storage* src = u.value ? value + u.t * v_st + u.head * v_sh : key + u.t * k_st + u.head * k_sh;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[16 * i] = static_cast<char>(w >> (8 * i));
-    if ((l & 3) == 0) rec[16 * d + d / 2 + (l >> 2) * 16 + tok] = static_cast<char>(byte);
+    for (int i = 0; i < GW; ++i) load8<T>(src + (u.group + i) * 32 + l * 8, u.value ? v_vec : k_vec, x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < GW; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < GW; ++i) {
+    const uint32_t byte = scale_byte(x[i], lo, hi);  // (the lanes of a token are there or not together)
+    const uint32_t w = quantise8(x[i], byte);
+    if (!rec) continue;
+    const int g = u.group + i;
+    if (!u.value) {
+      *reinterpret_cast<uint32_t*>(rec + tok * (d / 2) + g * 16 + l * 4) = w;
+      if (l == 0) rec[16 * d + g * 16 + (tok & 3) * 4 + (tok >> 2)] = static_cast<char>(byte);
+    } else {
+      char* v = rec + 8 * d + g * 256 + l * 64 + tok;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[16 * j] = static_cast<char>(w >> (8 * j));
+      if (l == 0) rec[16 * d + d / 2 + g * 16 + tok] = static_cast<char>(byte);
+    }
   }
 }
 
@@ -175,42 +207,53 @@ __device__ inline u32x4 codes8(uint32_t w, float s) {
 // else of it; 255 makes them return NaN).
 __device__ inline float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// A lane writes 8 elements of one (slot, head) row of K or V.
-template <class T, typename SlotT>
+// The append's units, read: a lane writes 8 elements of a group.
+template <class T, typename SlotT, int GW>
 __global__ void __launch_bounds__(256)
-read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t per_kv, int32_t lanes_per_row,
+read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int32_t groups, int64_t units,
                  typename T::storage* __restrict__ key, typename T::storage* __restrict__ value) {
-  int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (idx >= 2 * per_kv) return;
-  const bool is_v = idx >= per_kv;
-  if (is_v) idx -= per_kv;
-  const int64_t row = idx / lanes_per_row;
-  const int l = static_cast<int>(idx - row * lanes_per_row);
-  const int64_t t = row / pool.heads;
-  const int h = static_cast<int>(row - t * pool.heads);
-  const int d = lanes_per_row * 8;
+  const Unit4 u = unit_of<GW>(tokens, pool.heads, groups, units);
+  if (!u.there) return;
+  const int l = (threadIdx.x & 63) >> 4, d = groups * 32;
   int tok = 0;
-  const char* rec = record_of(pool, static_cast<int64_t>(slots[t]), h, tok);
-  uint32_t w = 0, byte = 127;
-  if (rec && !is_v) {
-    w = *reinterpret_cast<const uint32_t*>(rec + tok * (d / 2) + l * 4);
-    byte = static_cast<uint8_t>(rec[16 * d + (l >> 2) * 16 + (tok & 3) * 4 + (tok >> 2)]);
-  } else if (rec) {
-    const uint8_t* v = reinterpret_cast<const uint8_t*>(rec) + 8 * d + l * 64 + tok;
+  const char* rec = record_of(pool, static_cast<int64_t>(slots[u.t]), u.head, tok);
+  uint32_t w[GW] = {}, byte[GW];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(v[16 * i]) << (8 * i);
-    byte = static_cast<uint8_t>(rec[16 * d + d / 2 + (l >> 2) * 16 + tok]);
+  for (int i = 0; i < GW; ++i) byte[i] = 127;
+  if (rec && !u.value) {
+#pragma unroll
+    for (int i = 0; i < GW; ++i) {
+      const int g = u.group + i;
+      w[i] = *reinterpret_cast<const uint32_t*>(rec + tok * (d / 2) + g * 16 + l * 4);
+      byte[i] = static_cast<uint8_t>(rec[16 * d + g * 16 + (tok & 3) * 4 + (tok >> 2)]);
+    }
+  } else if (rec) {
+#pragma unroll
+    for (int i = 0; i < GW; ++i) {
+      const int g = u.group + i;
+      const uint8_t* v = reinterpret_cast<const uint8_t*>(rec) + 8 * d + g * 256 + l * 64 + tok;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i] |= static_cast<uint32_t>(v[16 * j]) << (8 * j);
+      byte[i] = static_cast<uint8_t>(rec[16 * d + d / 2 + g * 16 + tok]);
+    }
   }
-  const float s = scale_of(byte);
-  typename T::storage* out = (is_v ? value : key) + row * d + l * 8;
-  if constexpr (std::is_same<T, F32>::value) {
-    const u32x4 x = codes8<BF16>(w, s);
-    T::store8(out, f32x4{BF16::low_float(x.x), BF16::high_float(x.x), BF16::low_float(x.y), BF16::high_float(x.y)},
-              f32x4{BF16::low_float(x.z), BF16::high_float(x.z), BF16::low_float(x.w), BF16::high_float(x.w)});
-  } else {
-    *reinterpret_cast<u32x4*>(out) = codes8<T>(w, s);
+  typename T::storage* out = (u.value ? value : key) + (u.t * pool.heads + u.head) * d + u.group * 32 + l * 8;
+#pragma unroll
+  for (int i = 0; i < GW; ++i) {
+    const float s = scale_of(byte[i]);
+    if constexpr (std::is_same<T, F32>::value) {
+      const u32x4 x = codes8<BF16>(w[i], s);
+      T::store8(out + i * 32, f32x4{BF16::low_float(x.x), BF16::high_float(x.x), BF16::low_float(x.y), BF16::high_float(x.y)},
+                f32x4{BF16::low_float(x.z), BF16::high_float(x.z), BF16::low_float(x.w), BF16::high_float(x.w)});
+    } else {
+      *reinterpret_cast<u32x4*>(out + i * 32) = codes8<T>(w[i], s);
+    }
   }
 }
+
+// Groups of a wave: a whole head where there are many tokens (a wave then has
+// its loads in flight together), one where there are few.
+static int groups_a_wave(int64_t tokens, int64_t d) { return tokens >= 512 ? static_cast<int>(d == 256 ? 4 : d / 32) : 1; }
 
 // --------------------------------------------------------------- attention --
 
@@ -741,49 +784,67 @@ attn_4bit_kernel(Attn4Args a) {
   }
 }
 
-// Joins the parts of the query blocks that were cut: one wave an m-row.
+// Joins the parts of the query blocks that were cut: one wave an m-row, eight
+// parts on their way at a time.
 template <class IO, int D, int ROWS>
 __global__ void __launch_bounds__(256)
 merge_4bit_kernel(Attn4Args a) {
+  constexpr int PER = (D + 63) / 64, AHEAD = 8;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t u = blockIdx.x;
+  const int quarter = static_cast<int>(u % (ROWS / 4));  // m-rows 4 * quarter + wave
+  u /= ROWS / 4;
   const int head = static_cast<int>(u % a.hkv);
   u /= a.hkv;
   const int qb = static_cast<int>(u % a.q_blocks);
   const int row = static_cast<int>(u / a.q_blocks);
   Block4 b;
-  if (!block_of<ROWS>(a, row, head, qb, b)) return;
+  const int m = quarter * 4 + wave;
+  if (!block_of<ROWS>(a, row, head, qb, b) || m >= b.rows) return;
   const int steps = (b.limit + kStep - 1) / kStep;
   const int parts = (steps + a.part_steps - 1) / a.part_steps;
-  if (parts <= 1) return;
-  for (int m = wave; m < b.rows; m += 4) {
-    const int mr = b.first + m;
-    const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
-    if (tok < 0 || tok >= a.total_query) continue;
-    const int64_t w0 = (static_cast<int64_t>(row) * a.q_blocks + qb) * a.parts * a.hkv + head;
-    float top = -INFINITY;
-    for (int p = 0; p < parts; ++p) {
-      const float l = a.ws_lse[(w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m];
-      top = l > top || l != l ? l : top;
+  const int mr = b.first + m;
+  const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
+  if (parts <= 1 || tok < 0 || tok >= a.total_query) return;
+  const int64_t w0 = (static_cast<int64_t>(row) * a.q_blocks + qb) * a.parts * a.hkv + head;
+  float ref = -INFINITY, sum = 0, x[PER] = {};
+  for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+    float l[AHEAD], y[AHEAD][PER];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int p = imin(p0 + k, parts - 1);
+      const int64_t w = (w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m;
+      l[k] = p0 + k < parts ? a.ws_lse[w] : -INFINITY;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) y[k][i] = i * 64 + lane < D ? a.ws_o[w * D + i * 64 + lane] : 0.0f;
     }
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0, x[(D + 63) / 64] = {};
-    for (int p = 0; p < parts; ++p) {
-      const int64_t w = ((w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m);
-      const float f = F32::exp2(a.ws_lse[w] - ref);
+    float top = ref;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) top = l[k] > top || l[k] != l[k] ? l[k] : top;
+    const float base = top == -INFINITY ? 0.0f : top;  // no key seen so far
+    const float keep = F32::exp2(ref - base);
+    ref = top;
+    sum *= keep;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] *= keep;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (p0 + k >= parts) break;
+      const float f = F32::exp2(l[k] - base);
       sum += f;
 #pragma unroll
-      for (int i = 0; i < (D + 63) / 64; ++i)
-        if (i * 64 + lane < D) x[i] += f * a.ws_o[w * D + i * 64 + lane];
+      for (int i = 0; i < PER; ++i) x[i] += f * y[k][i];
     }
-    const float inv = sum == 0 ? 0.0f : 1.0f / sum;
-    typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + hd * a.o_sh;
-#pragma unroll
-    for (int i = 0; i < (D + 63) / 64; ++i)
-      if (i * 64 + lane < D) o[i * 64 + lane] = IO::from_float(x[i] * inv);
-    if (a.lse && lane == 0) a.lse[tok * a.l_st + hd * a.l_sh] = sum == 0 ? -INFINITY : (ref + F32::log2(sum)) * kLn2;
   }
+  const float inv = sum == 0 ? 0.0f : 1.0f / sum;
+  typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + hd * a.o_sh;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    if (i * 64 + lane < D) o[i * 64 + lane] = IO::from_float(x[i] * inv);
+  if (a.lse && lane == 0) a.lse[tok * a.l_st + hd * a.l_sh] = sum == 0 ? -INFINITY : (ref + F32::log2(sum)) * kLn2;
 }
+
+constexpr int64_t kWholeSteps = 64;
 
 // Split of a call: the query block's m-rows, key steps of a part, parts.
 struct Split4 {
@@ -796,11 +857,14 @@ static Split4 split_4bit(int64_t rows, int64_t max_q, int64_t max_k, int64_t gro
   s.mt = max_q * group > 16 && dtype != KVHOT_F32 && d <= 128 ? 2 : 1;
   s.q_blocks = static_cast<int32_t>((max_q * group + 16 * s.mt - 1) / (16 * s.mt));
   const int64_t steps = (max_k + kStep - 1) / kStep;
-  // Work-groups enough for four on each of 256 CUs, with two steps a wave at
-  // least.
+  // Blocks that give each of 256 CUs two work-groups are left whole up to
+  // kWholeSteps steps (64 rows of 128-2048 keys: 23.6 us, in two parts 25.7 and
+  // a merge of 4.8); fewer are cut for four work-groups a CU, of which three
+  // fit: rows are ragged, and the parts behind a short row's end are empty
+  // (24 rows of up to 6000 keys: 20.9 us, 24.9 when cut for three).
   const int64_t blocks = rows * s.q_blocks * hkv;
-  int64_t parts = std::max<int64_t>(1, (1024 + blocks - 1) / blocks);
-  int64_t per = std::max<int64_t>((steps + parts - 1) / parts, 2 * kWaves4);
+  const int64_t parts = blocks >= 512 ? 1 : (1024 + blocks - 1) / blocks;
+  const int64_t per = std::min<int64_t>(std::max<int64_t>((steps + parts - 1) / parts, 2 * kWaves4), kWholeSteps);
   s.part_steps = static_cast<int32_t>(std::max<int64_t>(per, 1));
   s.parts = static_cast<int32_t>(std::max<int64_t>((steps + per - 1) / per, 1));
   s.ws_bytes = s.parts > 1 ? blocks * s.parts * 16 * s.mt * (d + 1) * 4 : 0;
@@ -840,6 +904,24 @@ static bool aligned(const void* p, int64_t es, int64_t unit, std::initializer_li
   return true;
 }
 
+// GO(T, slot type, groups a wave) for this call's dtype, slots and gw.
+#define KVHOT_FOR_GROUPS(GO, T, S)   \
+  switch (gw) {                      \
+    case 1: GO(T, S, 1); break;      \
+    case 2: GO(T, S, 2); break;      \
+    case 3: GO(T, S, 3); break;      \
+    default: GO(T, S, 4); break;     \
+  }
+#define KVHOT_FOR_TYPES(GO)                                           \
+  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {                      \
+    case KVHOT_F32 * 2: KVHOT_FOR_GROUPS(GO, F32, int32_t) break;     \
+    case KVHOT_F32 * 2 + 1: KVHOT_FOR_GROUPS(GO, F32, int64_t) break; \
+    case KVHOT_F16 * 2: KVHOT_FOR_GROUPS(GO, F16, int32_t) break;     \
+    case KVHOT_F16 * 2 + 1: KVHOT_FOR_GROUPS(GO, F16, int64_t) break; \
+    case KVHOT_BF16 * 2: KVHOT_FOR_GROUPS(GO, BF16, int32_t) break;   \
+    default: KVHOT_FOR_GROUPS(GO, BF16, int64_t) break;               \
+  }
+
 extern "C" int kvhot_reshape_and_cache_4bit(
     const void* key, const int64_t key_strides[3], const void* value, const int64_t value_strides[3], void* cache,
     int64_t block_stride_bytes, const void* slot_mapping, int slot_is_int64, int64_t num_tokens, int64_t num_kv_heads,
@@ -857,27 +939,20 @@ extern "C" int kvhot_reshape_and_cache_4bit(
     return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: head_dim must be the innermost, unit-stride dim");
   if (reinterpret_cast<uintptr_t>(key) % es || reinterpret_cast<uintptr_t>(value) % es)
     return set_error(KVHOT_EINVAL, "reshape_and_cache_4bit: misaligned tensors");
-  const int64_t per_kv = num_tokens * num_kv_heads * (head_dim / 8);
-  const int64_t groups = (2 * per_kv + 255) / 256;
-  if (groups > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "reshape_and_cache_4bit: too many tokens");
+  const int gw = groups_a_wave(num_tokens, head_dim);
+  const int64_t units = (num_tokens + 15) / 16 * num_kv_heads * 2 * (head_dim / 32 / gw);
+  if ((units + 3) / 4 > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "reshape_and_cache_4bit: too many tokens");
   const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
   const int kv = aligned(key, es, 16, {key_strides[0], key_strides[1]});
   const int vv = aligned(value, es, 16, {value_strides[0], value_strides[1]});
-#define KVHOT_GO(T, S)                                                                                               \
-  hipLaunchKernelGGL((append_4bit_kernel<T, S>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0,                   \
+#define KVHOT_LAUNCH(T, S, GW)                                                                                        \
+  hipLaunchKernelGGL((append_4bit_kernel<T, S, GW>), dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,      \
                      static_cast<hipStream_t>(stream), static_cast<const T::storage*>(key),                           \
-                     static_cast<const T::storage*>(value), pool, static_cast<const S*>(slot_mapping), per_kv,        \
-                     static_cast<int32_t>(head_dim / 8), key_strides[0], key_strides[1], value_strides[0],            \
+                     static_cast<const T::storage*>(value), pool, static_cast<const S*>(slot_mapping), num_tokens,    \
+                     static_cast<int32_t>(head_dim / 32), units, key_strides[0], key_strides[1], value_strides[0],    \
                      value_strides[1], kv, vv, scale_lo(dtype), scale_hi(dtype))
-  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {
-    case KVHOT_F32 * 2: KVHOT_GO(F32, int32_t); break;
-    case KVHOT_F32 * 2 + 1: KVHOT_GO(F32, int64_t); break;
-    case KVHOT_F16 * 2: KVHOT_GO(F16, int32_t); break;
-    case KVHOT_F16 * 2 + 1: KVHOT_GO(F16, int64_t); break;
-    case KVHOT_BF16 * 2: KVHOT_GO(BF16, int32_t); break;
-    default: KVHOT_GO(BF16, int64_t); break;
-  }
-#undef KVHOT_GO
+  KVHOT_FOR_TYPES(KVHOT_LAUNCH)
+#undef KVHOT_LAUNCH
   return launch_status("reshape_and_cache_4bit");
 }
 
@@ -893,23 +968,17 @@ extern "C" int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_byt
   if (!key || !value || !slots) return set_error(KVHOT_EINVAL, "read_cache_4bit: null pointer");
   if (reinterpret_cast<uintptr_t>(key) % 16 || reinterpret_cast<uintptr_t>(value) % 16)
     return set_error(KVHOT_EINVAL, "read_cache_4bit: misaligned tensors");
-  const int64_t per_kv = num_slots * num_kv_heads * (head_dim / 8);
-  const int64_t groups = (2 * per_kv + 255) / 256;
-  if (groups > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "read_cache_4bit: too many slots");
+  const int gw = groups_a_wave(num_slots, head_dim);
+  const int64_t units = (num_slots + 15) / 16 * num_kv_heads * 2 * (head_dim / 32 / gw);
+  if ((units + 3) / 4 > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "read_cache_4bit: too many slots");
   const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
-#define KVHOT_GO(T, S)                                                                                             \
-  hipLaunchKernelGGL((read_4bit_kernel<T, S>), dim3(static_cast<uint32_t>(groups)), dim3(256), 0,                   \
-                     static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), per_kv,                  \
-                     static_cast<int32_t>(head_dim / 8), static_cast<T::storage*>(key), static_cast<T::storage*>(value))
-  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {
-    case KVHOT_F32 * 2: KVHOT_GO(F32, int32_t); break;
-    case KVHOT_F32 * 2 + 1: KVHOT_GO(F32, int64_t); break;
-    case KVHOT_F16 * 2: KVHOT_GO(F16, int32_t); break;
-    case KVHOT_F16 * 2 + 1: KVHOT_GO(F16, int64_t); break;
-    case KVHOT_BF16 * 2: KVHOT_GO(BF16, int32_t); break;
-    default: KVHOT_GO(BF16, int64_t); break;
-  }
-#undef KVHOT_GO
+#define KVHOT_LAUNCH(T, S, GW)                                                                                      \
+  hipLaunchKernelGGL((read_4bit_kernel<T, S, GW>), dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,      \
+                     static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), num_slots,               \
+                     static_cast<int32_t>(head_dim / 32), units, static_cast<T::storage*>(key),                     \
+                     static_cast<T::storage*>(value))
+  KVHOT_FOR_TYPES(KVHOT_LAUNCH)
+#undef KVHOT_LAUNCH
   return launch_status("read_cache_4bit");
 }
 
@@ -940,12 +1009,13 @@ namespace {
 template <class IO, class M, int NP, int D, int MT>
 int launch_4bit(const Attn4Args& a, int64_t rows, hipStream_t s) {
   const int64_t blocks = rows * a.q_blocks * a.hkv;
-  if (blocks * a.parts > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
+  if (blocks * std::max<int64_t>(a.parts, 4 * MT) > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
   hipLaunchKernelGGL((attn_4bit_kernel<IO, M, NP, D, MT>), dim3(static_cast<uint32_t>(blocks * a.parts)),
                      dim3(64 * kWaves4), 0, s, a);
   if (int e = launch_status("paged_attention_4bit")) return e;
   if (a.parts > 1) {
-    hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks * (4 * MT))),
+                       dim3(256), 0, s, a);
     return launch_status("paged_attention_4bit merge");
   }
   return 0;
