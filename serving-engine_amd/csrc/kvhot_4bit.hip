@@ -207,7 +207,9 @@ __device__ inline u32x4 codes8(uint32_t w, float s) {
 // else of it; 255 makes them return NaN).
 __device__ inline float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// The append's units, read: a lane writes 8 elements of a group.
+// The append's units, read: a lane writes 8 elements of a group, past the caches
+// (90k tokens of 8 heads, 480 MB in all: 106 us = 4.5 TB/s, 165 with ordinary
+// stores).
 template <class T, typename SlotT, int GW>
 __global__ void __launch_bounds__(256)
 read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int32_t groups, int64_t units,
@@ -243,10 +245,13 @@ read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, in
     const float s = scale_of(byte[i]);
     if constexpr (std::is_same<T, F32>::value) {
       const u32x4 x = codes8<BF16>(w[i], s);
-      T::store8(out + i * 32, f32x4{BF16::low_float(x.x), BF16::high_float(x.x), BF16::low_float(x.y), BF16::high_float(x.y)},
-                f32x4{BF16::low_float(x.z), BF16::high_float(x.z), BF16::low_float(x.w), BF16::high_float(x.w)});
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        __builtin_nontemporal_store(f32x4{BF16::low_float(x[2 * h]), BF16::high_float(x[2 * h]),
+                                          BF16::low_float(x[2 * h + 1]), BF16::high_float(x[2 * h + 1])},
+                                    reinterpret_cast<f32x4*>(out + i * 32 + 4 * h));
     } else {
-      *reinterpret_cast<u32x4*>(out + i * 32) = codes8<T>(w[i], s);
+      __builtin_nontemporal_store(codes8<T>(w[i], s), reinterpret_cast<u32x4*>(out + i * 32));
     }
   }
 }

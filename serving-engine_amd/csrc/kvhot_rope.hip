@@ -40,10 +40,16 @@ __device__ inline f32x4 load4(const typename T::storage* p, bool vec) {
   }
 }
 
-template <class T>
+// PAST: past the caches.
+template <class T, bool PAST>
 __device__ inline void put4(typename T::storage* p, f32x4 x, bool vec) {
   if (vec) {
-    T::store4(p, x);
+    if constexpr (!PAST)
+      T::store4(p, x);
+    else if constexpr (sizeof(typename T::storage) == 2)
+      __builtin_nontemporal_store(u32x2{T::pack2(x.x, x.y), T::pack2(x.z, x.w)}, reinterpret_cast<u32x2*>(p));
+    else
+      __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(p));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) p[i] = T::from_float(x[i]);
@@ -132,8 +138,8 @@ norm_rope_kernel(RopeArgs a) {
     if (in && h < heads) {
       S* y = h < a.hq ? static_cast<S*>(a.q_out) + t * a.qo_st + h * a.qo_sh
                       : static_cast<S*>(a.k_out) + t * a.ko_st + (h - a.hq) * a.ko_sh;
-      put4<T>(y + ea, ya, a.vec);
-      put4<T>(y + eb, yb, a.vec);
+      put4<T, (U > 1)>(y + ea, ya, a.vec);
+      put4<T, (U > 1)>(y + eb, yb, a.vec);
     }
   }
 }
@@ -150,6 +156,17 @@ static int launch_rope(const RopeArgs& a, hipStream_t s) {
 
 template <class T>
 static int launch_rope(const RopeArgs& a, hipStream_t s) {
+  // Outputs that pass the 8 L2s' 32 MiB: two sets of heads a wave, stored past
+  // the caches (8192 tokens of 40 heads of 128, bf16, 168 MB: 35.0 us = 4.8 TB/s;
+  // one set and ordinary stores 41.2, two 37.5, five 39.8, five past the caches
+  // 36.2).  Below that what is stored is read soon, and one set gives more waves.
+  const int64_t bytes = a.tokens * (a.hq + a.hkv) * a.d * static_cast<int64_t>(sizeof(typename T::storage));
+  if (bytes >= (int64_t{32} << 20)) {
+    if (a.d <= 64) return launch_rope<T, 8, 2>(a, s);
+    if (a.d <= 128) return launch_rope<T, 16, 2>(a, s);
+    if (a.d <= 256) return launch_rope<T, 32, 2>(a, s);
+    return launch_rope<T, 64, 2>(a, s);
+  }
   if (a.d <= 64) return launch_rope<T, 8, 1>(a, s);
   if (a.d <= 128) return launch_rope<T, 16, 1>(a, s);
   if (a.d <= 256) return launch_rope<T, 32, 1>(a, s);

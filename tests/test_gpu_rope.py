@@ -51,6 +51,25 @@ def test_against_64_bits(cuda, sea, dtype, d, rotary, interleaved, norm, t, hq, 
     assert a is q and torch.equal(q, oq) and torch.equal(k, ok)
 
 
+@pytest.mark.parametrize("dtype,d,t", [(BF16, 128, 8192), (FP32, 64, 8195), (FP16, 256, 4100), (BF16, 512, 1700)])
+def test_long_prompts(cuda, sea, dtype, d, t):
+    """Outputs beyond 32 MiB take two sets of heads a wave: 21 heads, an odd count."""
+    print("case: norm_rope long", dtype, d, t, flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    qkv = torch.randn(t, 21, d, generator=gen, device=cuda).to(dtype)
+    w = (1 + 0.3 * torch.randn(2, d, generator=gen, device=cuda)).to(dtype)
+    pos, table = torch.arange(t, device=cuda), sea.rope_table(t, d)
+    oq, ok = sea.norm_rope(qkv[:, :17], qkv[:, 17:], pos, table, w[0], w[1])
+    for s in (slice(0, 70), slice(t // 2, t // 2 + 70), slice(t - 70, t)):
+        check(oq[s], qkv[s, :17], w[0], pos[s], table, False)
+        check(ok[s], qkv[s, 17:], w[1], pos[s], table, False)
+    # every row the same as in small calls, in place too
+    parts = [sea.norm_rope(qkv[i:i + 500, :17], qkv[i:i + 500, 17:], pos[i:i + 500], table, w[0], w[1]) for i in range(0, t, 500)]
+    assert torch.equal(oq, torch.cat([p[0] for p in parts])) and torch.equal(ok, torch.cat([p[1] for p in parts]))
+    sea.norm_rope(qkv[:, :17], qkv[:, 17:], pos, table, w[0], w[1], out=(qkv[:, :17], qkv[:, 17:]))
+    assert torch.equal(qkv[:, :17], oq) and torch.equal(qkv[:, 17:], ok)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 def test_layouts_weights_and_no_heads(cuda, sea, dtype):
     table = sea.rope_table(64, 64)
