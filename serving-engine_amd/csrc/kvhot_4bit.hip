@@ -207,41 +207,72 @@ __device__ inline u32x4 codes8(uint32_t w, float s) {
 // else of it; 255 makes them return NaN).
 __device__ inline float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// The append's units, read: a lane writes 8 elements of a group, past the caches
-// (90k tokens of 8 heads, 480 MB in all: 106 us = 4.5 TB/s, 165 with ordinary
-// stores).
-template <class T, typename SlotT, int GW>
+// A wave reads 16 slots of one head, K or V.  It writes whole rows, D / 8 lanes a
+// row, past the caches; K's codes are read in that order too.  V's are read as the
+// append writes them, tokens side by side, and change lanes in LDS: with 64-byte
+// pieces of 16 rows in a store instead, 90k tokens (480 MB in all) took 192 us
+// from HBM.
+template <class T, typename SlotT, int D>
 __global__ void __launch_bounds__(256)
-read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int32_t groups, int64_t units,
+read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int64_t units,
                  typename T::storage* __restrict__ key, typename T::storage* __restrict__ value) {
-  const Unit4 u = unit_of<GW>(tokens, pool.heads, groups, units);
-  if (!u.there) return;
-  const int l = (threadIdx.x & 63) >> 4, d = groups * 32;
+  constexpr int CH = D / 8, NI = D / 32;  // 8-element chunks of a row; chunks of a lane
+  __shared__ uint32_t codes[4][16 * (CH + 1)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t u = static_cast<int64_t>(blockIdx.x) * 4 + wave;
+  const bool there = u < units;  // (every wave meets the barrier)
+  const bool is_v = u & 1;
+  u >>= 1;
+  const int head = static_cast<int>(u % pool.heads);
+  const int64_t t0 = u / pool.heads * 16;
   int tok = 0;
-  const char* rec = record_of(pool, static_cast<int64_t>(slots[u.t]), u.head, tok);
-  uint32_t w[GW] = {}, byte[GW];
+  const int64_t mine = t0 + (lane & 15);
+  const char* rec = there && mine < tokens ? record_of(pool, static_cast<int64_t>(slots[mine]), head, tok) : nullptr;
+  uint32_t w[NI], byte[NI];
 #pragma unroll
-  for (int i = 0; i < GW; ++i) byte[i] = 127;
-  if (rec && !u.value) {
+  for (int i = 0; i < NI; ++i) w[i] = 0;
+  if (is_v && rec) {
+    const int l = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < GW; ++i) {
-      const int g = u.group + i;
-      w[i] = *reinterpret_cast<const uint32_t*>(rec + tok * (d / 2) + g * 16 + l * 4);
-      byte[i] = static_cast<uint8_t>(rec[16 * d + g * 16 + (tok & 3) * 4 + (tok >> 2)]);
-    }
-  } else if (rec) {
-#pragma unroll
-    for (int i = 0; i < GW; ++i) {
-      const int g = u.group + i;
-      const uint8_t* v = reinterpret_cast<const uint8_t*>(rec) + 8 * d + g * 256 + l * 64 + tok;
+    for (int i = 0; i < NI; ++i) {
+      const uint8_t* v = reinterpret_cast<const uint8_t*>(rec) + 8 * D + i * 256 + l * 64 + tok;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[i] |= static_cast<uint32_t>(v[16 * j]) << (8 * j);
-      byte[i] = static_cast<uint8_t>(rec[16 * d + d / 2 + g * 16 + tok]);
     }
   }
-  typename T::storage* out = (u.value ? value : key) + (u.t * pool.heads + u.head) * d + u.group * 32 + l * 8;
+  const uint64_t at = reinterpret_cast<uint64_t>(rec);
+  const int lo = static_cast<int>(at), hi = static_cast<int>(at >> 32);
 #pragma unroll
-  for (int i = 0; i < GW; ++i) {
+  for (int i = 0; i < NI; ++i) {
+    const int t = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH;
+    const uint64_t r = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, t, kWave))) << 32 |
+                       static_cast<uint32_t>(__shfl(lo, t, kWave));
+    const int tk = __shfl(tok, t, kWave);
+    const char* p = reinterpret_cast<const char*>(r);
+    byte[i] = 127;
+    if (p && is_v) {
+      byte[i] = static_cast<uint8_t>(p[16 * D + D / 2 + (c >> 2) * 16 + tk]);
+    } else if (p) {
+      w[i] = *reinterpret_cast<const uint32_t*>(p + tk * (D / 2) + c * 4);
+      byte[i] = static_cast<uint8_t>(p[16 * D + (c >> 2) * 16 + (tk & 3) * 4 + (tk >> 2)]);
+    }
+  }
+  uint32_t* own = codes[wave];
+  if (is_v) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) own[(lane & 15) * (CH + 1) + i * 4 + (lane >> 4)] = w[i];
+  }
+  __syncthreads();
+  if (is_v) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) w[i] = own[(i * 64 + lane) / CH * (CH + 1) + (i * 64 + lane) % CH];
+  }
+  typename T::storage* out = is_v ? value : key;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int t = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH;
+    if (!there || t0 + t >= tokens) continue;
+    typename T::storage* o = out + ((t0 + t) * pool.heads + head) * D + c * 8;
     const float s = scale_of(byte[i]);
     if constexpr (std::is_same<T, F32>::value) {
       const u32x4 x = codes8<BF16>(w[i], s);
@@ -249,9 +280,9 @@ read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, in
       for (int h = 0; h < 2; ++h)
         __builtin_nontemporal_store(f32x4{BF16::low_float(x[2 * h]), BF16::high_float(x[2 * h]),
                                           BF16::low_float(x[2 * h + 1]), BF16::high_float(x[2 * h + 1])},
-                                    reinterpret_cast<f32x4*>(out + i * 32 + 4 * h));
+                                    reinterpret_cast<f32x4*>(o + 4 * h));
     } else {
-      __builtin_nontemporal_store(codes8<T>(w[i], s), reinterpret_cast<u32x4*>(out + i * 32));
+      __builtin_nontemporal_store(codes8<T>(w[i], s), reinterpret_cast<u32x4*>(o));
     }
   }
 }
@@ -909,22 +940,29 @@ static bool aligned(const void* p, int64_t es, int64_t unit, std::initializer_li
   return true;
 }
 
-// GO(T, slot type, groups a wave) for this call's dtype, slots and gw.
-#define KVHOT_FOR_GROUPS(GO, T, S)   \
-  switch (gw) {                      \
-    case 1: GO(T, S, 1); break;      \
-    case 2: GO(T, S, 2); break;      \
-    case 3: GO(T, S, 3); break;      \
-    default: GO(T, S, 4); break;     \
+// GO(T, slot type, N) for this call's dtype and slots, N groups a wave or the head_dim.
+#define KVHOT_FOR_GROUPS(GO, T, S) \
+  switch (gw) {                    \
+    case 1: GO(T, S, 1); break;    \
+    case 2: GO(T, S, 2); break;    \
+    case 3: GO(T, S, 3); break;    \
+    default: GO(T, S, 4); break;   \
   }
-#define KVHOT_FOR_TYPES(GO)                                           \
-  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {                      \
-    case KVHOT_F32 * 2: KVHOT_FOR_GROUPS(GO, F32, int32_t) break;     \
-    case KVHOT_F32 * 2 + 1: KVHOT_FOR_GROUPS(GO, F32, int64_t) break; \
-    case KVHOT_F16 * 2: KVHOT_FOR_GROUPS(GO, F16, int32_t) break;     \
-    case KVHOT_F16 * 2 + 1: KVHOT_FOR_GROUPS(GO, F16, int64_t) break; \
-    case KVHOT_BF16 * 2: KVHOT_FOR_GROUPS(GO, BF16, int32_t) break;   \
-    default: KVHOT_FOR_GROUPS(GO, BF16, int64_t) break;               \
+#define KVHOT_FOR_DIMS(GO, T, S)   \
+  switch (head_dim) {              \
+    case 64: GO(T, S, 64); break;  \
+    case 96: GO(T, S, 96); break;  \
+    case 128: GO(T, S, 128); break; \
+    default: GO(T, S, 256); break; \
+  }
+#define KVHOT_FOR_TYPES(GO, FOR)                          \
+  switch (dtype * 2 + (slot_is_int64 ? 1 : 0)) {          \
+    case KVHOT_F32 * 2: FOR(GO, F32, int32_t) break;      \
+    case KVHOT_F32 * 2 + 1: FOR(GO, F32, int64_t) break;  \
+    case KVHOT_F16 * 2: FOR(GO, F16, int32_t) break;      \
+    case KVHOT_F16 * 2 + 1: FOR(GO, F16, int64_t) break;  \
+    case KVHOT_BF16 * 2: FOR(GO, BF16, int32_t) break;    \
+    default: FOR(GO, BF16, int64_t) break;                \
   }
 
 extern "C" int kvhot_reshape_and_cache_4bit(
@@ -956,7 +994,7 @@ extern "C" int kvhot_reshape_and_cache_4bit(
                      static_cast<const T::storage*>(value), pool, static_cast<const S*>(slot_mapping), num_tokens,    \
                      static_cast<int32_t>(head_dim / 32), units, key_strides[0], key_strides[1], value_strides[0],    \
                      value_strides[1], kv, vv, scale_lo(dtype), scale_hi(dtype))
-  KVHOT_FOR_TYPES(KVHOT_LAUNCH)
+  KVHOT_FOR_TYPES(KVHOT_LAUNCH, KVHOT_FOR_GROUPS)
 #undef KVHOT_LAUNCH
   return launch_status("reshape_and_cache_4bit");
 }
@@ -973,16 +1011,14 @@ extern "C" int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_byt
   if (!key || !value || !slots) return set_error(KVHOT_EINVAL, "read_cache_4bit: null pointer");
   if (reinterpret_cast<uintptr_t>(key) % 16 || reinterpret_cast<uintptr_t>(value) % 16)
     return set_error(KVHOT_EINVAL, "read_cache_4bit: misaligned tensors");
-  const int gw = groups_a_wave(num_slots, head_dim);
-  const int64_t units = (num_slots + 15) / 16 * num_kv_heads * 2 * (head_dim / 32 / gw);
+  const int64_t units = (num_slots + 15) / 16 * num_kv_heads * 2;
   if ((units + 3) / 4 > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "read_cache_4bit: too many slots");
   const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
-#define KVHOT_LAUNCH(T, S, GW)                                                                                      \
-  hipLaunchKernelGGL((read_4bit_kernel<T, S, GW>), dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,      \
-                     static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), num_slots,               \
-                     static_cast<int32_t>(head_dim / 32), units, static_cast<T::storage*>(key),                     \
-                     static_cast<T::storage*>(value))
-  KVHOT_FOR_TYPES(KVHOT_LAUNCH)
+#define KVHOT_LAUNCH(T, S, D)                                                                                    \
+  hipLaunchKernelGGL((read_4bit_kernel<T, S, D>), dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,    \
+                     static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), num_slots, units,     \
+                     static_cast<T::storage*>(key), static_cast<T::storage*>(value))
+  KVHOT_FOR_TYPES(KVHOT_LAUNCH, KVHOT_FOR_DIMS)
 #undef KVHOT_LAUNCH
   return launch_status("read_cache_4bit");
 }
