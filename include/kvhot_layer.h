@@ -96,6 +96,9 @@ int kvhot_norm_rope(const void* q, const int64_t q_strides[3], const void* k,
  * kvhot_read_cache_4bit: key[i], value[i] (contiguous [num_slots,
  * num_kv_heads, head_dim], 16-byte aligned) = what the cache holds at slots[i], exact in
  * every dtype for values appended from it (zeros for a slot outside the pool).
+ * as_blocks: into kv-interleaved blocks instead, for an attention over the copies:
+ * key is [num_slots / 16, num_kv_heads, 2, 16, head_dim] (K, then V; value is not
+ * used), num_slots a multiple of 16, and NaN reads as 0 (kvhot_spread_nan_4bit).
  */
 int kvhot_reshape_and_cache_4bit(
     const void* key, const int64_t key_strides[3], const void* value,
@@ -107,8 +110,8 @@ int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_bytes,
                           const void* slots, int slot_is_int64,
                           int64_t num_slots, int64_t num_kv_heads,
                           int64_t head_dim, int64_t block_size,
-                          int64_t num_blocks, void* key, void* value, int dtype,
-                          void* stream);
+                          int64_t num_blocks, void* key, void* value,
+                          int as_blocks, int dtype, void* stream);
 
 /*
  * kvhot_paged_attention over a cache held in 4 bits: the same rows, masking
@@ -135,6 +138,24 @@ int kvhot_paged_attention_4bit(
     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
     int64_t block_size, int64_t num_blocks, float scale, int attn_flags,
     int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * For prompts that are attended over dense copies of their keys
+ * (kvhot_read_cache_4bit with as_blocks, then kvhot_paged_attention): writes NaN
+ * into the outputs of the queries that see a NaN of the cache.  Row r of the
+ * arrays is row rows[r] of block_table; for each of its queries, a NaN in a
+ * visible K makes its heads' out and lse NaN, one in a visible V the 32
+ * elements of out that share its scale.
+ */
+int kvhot_spread_nan_4bit(
+    const void* cache, int64_t block_stride_bytes, void* out,
+    const int64_t out_strides[3], float* lse, const int64_t lse_strides[2],
+    const int32_t* block_table, int64_t bt_row_stride, const int32_t* rows,
+    const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_starts,
+    const int32_t* q_pos_offsets, int64_t num_rows, int64_t total_query,
+    int64_t max_q_len, int64_t max_k_len, int64_t num_q_heads,
+    int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+    int64_t num_blocks, int attn_flags, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -85,7 +85,7 @@ SIGNATURES = {
     ),
 }
 
-# The same for include/kvhot_layer.h, in its order (bind_layer's).
+# The same for include/kvhot_layer.h.
 LAYER_SIGNATURES = {
     "kvhot_build_block_tables": (
         _int,
@@ -102,7 +102,7 @@ LAYER_SIGNATURES = {
     ),
     "kvhot_read_cache_4bit": (
         _int,
-        [_vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp],
+        [_vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _int, _int, _vp],
     ),
     "kvhot_paged_attention_4bit_workspace_bytes": (
         _i64,
@@ -112,6 +112,11 @@ LAYER_SIGNATURES = {
         _int,
         [_vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _int, _vp, _i64, _vp],
+    ),
+    "kvhot_spread_nan_4bit": (
+        _int,
+        [_vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+         _i64, _i64, _int, _int, _vp],
     ),
 }
 
@@ -157,7 +162,9 @@ def native():
                               "`python serving-engine_amd/build.py`") from e
         kvhot_torch.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "kvhot_paged_attention", "kvhot_paged_attention_workspace_bytes", "kvhot_reshape_and_cache")))
-        kvhot_torch.bind_layer(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in LAYER_SIGNATURES))
+        kvhot_torch.bind_layer(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "kvhot_build_block_tables", "kvhot_norm_rope", "kvhot_reshape_and_cache_4bit", "kvhot_read_cache_4bit",
+            "kvhot_paged_attention_4bit_workspace_bytes", "kvhot_paged_attention_4bit")))
         _NATIVE = kvhot_torch
     return _NATIVE
 

@@ -216,12 +216,22 @@ __device__ inline float scale_in(uint32_t word, int i) {
   return __uint_as_float(i == 3 ? word >> 1 : word << (23 - 8 * i));
 }
 
+template <bool CACHED, class V>
+__device__ inline void put(V x, void* p) {
+  if constexpr (CACHED)
+    *static_cast<V*>(p) = x;
+  else
+    __builtin_nontemporal_store(x, static_cast<V*>(p));
+}
+
 // A wave reads 16 slots of one head, K or V.  It writes whole rows, D / 8 lanes a
 // row, past the caches; K's codes are read in that order too.  V's are read as the
 // append writes them, tokens side by side, and change lanes in LDS: with 64-byte
 // pieces of 16 rows in a store instead, 90k tokens (480 MB in all) took 192 us
 // from HBM.
-template <class T, typename SlotT, int D>
+// BLOCKS: into kv-interleaved blocks of 16 tokens at `key` instead, NaN as 0, and
+// stored where the next kernel finds them.
+template <class T, typename SlotT, int D, bool BLOCKS>
 __global__ void __launch_bounds__(256)
 read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, int64_t units,
                  typename T::storage* __restrict__ key, typename T::storage* __restrict__ value) {
@@ -281,17 +291,22 @@ read_4bit_kernel(Pool4 pool, const SlotT* __restrict__ slots, int64_t tokens, in
   for (int i = 0; i < NI; ++i) {
     const int t = (i * 64 + lane) / CH, c = (i * 64 + lane) % CH;
     if (!there || t0 + t >= tokens) continue;
-    typename T::storage* o = out + ((t0 + t) * pool.heads + head) * D + c * 8;
+    typename T::storage* o = BLOCKS ? key + ((t0 / 16 * pool.heads + head) * 2 + (is_v ? 1 : 0)) * (16 * D) + t * D + c * 8
+                                    : out + ((t0 + t) * pool.heads + head) * D + c * 8;
+    if (BLOCKS && byte[i] == 255) {
+      byte[i] = 127;
+      w[i] = 0;
+    }
     const float s = scale_of(byte[i]);
     if constexpr (std::is_same<T, F32>::value) {
       const u32x4 x = codes8<BF16>(w[i], s);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        __builtin_nontemporal_store(f32x4{BF16::low_float(x[2 * h]), BF16::high_float(x[2 * h]),
-                                          BF16::low_float(x[2 * h + 1]), BF16::high_float(x[2 * h + 1])},
-                                    reinterpret_cast<f32x4*>(o + 4 * h));
+        put<BLOCKS>(f32x4{BF16::low_float(x[2 * h]), BF16::high_float(x[2 * h]), BF16::low_float(x[2 * h + 1]),
+                          BF16::high_float(x[2 * h + 1])},
+                    o + 4 * h);
     } else {
-      __builtin_nontemporal_store(codes8<T>(w[i], s), reinterpret_cast<u32x4*>(o));
+      put<BLOCKS>(codes8<T>(w[i], s), o);
     }
   }
 }
@@ -318,7 +333,7 @@ struct Attn4Args {
   int32_t num_rows, hq, hkv, group, block_size, num_blocks, causal;
   float scale;     // |scale| * log2(e)
   int32_t negate;  // the scale is negative: Q's sign is turned
-  int32_t q_vec, o_vec;
+  int32_t q_vec;
   // the padded grid
   int32_t q_blocks, parts, part_steps, max_q, max_k, spb;
   int64_t blocks;  // query blocks of the grid
@@ -592,22 +607,23 @@ __device__ inline float highest(f32x4 a, f32x4 b) {
   return highest(highest(highest(highest(a[0], a[1]), a[2]), highest(highest(a[3], b[0]), b[1])), highest(b[2], b[3]));
 }
 
-// Probabilities from scores: lane (n, g) holds m-row n's for the 16 keys key(t, r),
-// the B operand of O^T's two products of 32 keys.  MASKED: some m-row does not see
+// Probabilities from scores: lane (n, g) holds m-row n's for the 16 keys first +
+// key(t, r) (first the lane's, key(t, r) known here), the B operand of O^T's two products of 32 keys.  MASKED: some m-row does not see
 // all 64 keys.
 template <class M, int NP, int D, int MT, bool MASKED, class K>
-__device__ inline void probabilities(f32x4 (&sc)[MT][4], const int (&sees)[MT], K key, float scale, State4<D, MT>& st,
-                                     u32x4 (&p)[MT][NP][2]) {
+__device__ inline void probabilities(f32x4 (&sc)[MT][4], const int (&sees)[MT], int first, K key, float scale,
+                                     State4<D, MT>& st, u32x4 (&p)[MT][NP][2]) {
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     // (A NaN passes through IEEE's maximum, which needs no canonical operands, and
     // then moves nothing: what the m-row comes to is NaN by that score alone.)
+    const int left = sees[m] - first;
     if (MASKED) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (key(t, r) >= sees[m]) sc[m][t][r] = -INFINITY;
+          if (key(t, r) >= left) sc[m][t][r] = -INFINITY;
     }
     float top = highest(highest(sc[m][0], sc[m][1]), highest(sc[m][2], sc[m][3]));
     if (__any(top * scale > st.above[m])) {
@@ -631,8 +647,8 @@ __device__ inline void probabilities(f32x4 (&sc)[MT][4], const int (&sees)[MT], 
       for (int r = 0; r < 4; r += 2) {
         float x = BF16::exp2(fmaf(sc[m][t][r], scale, -st.ref[m])), y = BF16::exp2(fmaf(sc[m][t][r + 1], scale, -st.ref[m]));
         if (MASKED) {  // (a scale of 0 would make NaN of them)
-          if (key(t, r) >= sees[m]) x = 0;
-          if (key(t, r + 1) >= sees[m]) y = 0;
+          if (key(t, r) >= left) x = 0;
+          if (key(t, r + 1) >= left) y = 0;
         }
         st.sum[m] += x + y;
         uint32_t w[NP];
@@ -664,7 +680,7 @@ __device__ inline void weigh(const Values4<D>& s, const u32x4 (&p)[MT][NP][2], c
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
         const uint32_t sh = 8 * (t & 3);
-        const bool seen = base + 16 * g + t < limit, nan = ((vs[c][t >> 2] >> sh) & 255) == 255;
+        const bool seen = t < limit - base - 16 * g, nan = ((vs[c][t >> 2] >> sh) & 255) == 255;
         if (seen && nan) bad[c] |= 1u << t;
         if (!seen || nan) vs[c][t >> 2] = (vs[c][t >> 2] & ~(255u << sh)) | 127u << sh;
       }
@@ -826,8 +842,8 @@ attn_4bit_kernel(Attn4Args a) {
       load_keys<D>(a, b, w, lane, keys);
       __builtin_amdgcn_sched_barrier(0);
       u32x4 p[MT][NP][2];
-      const auto key = [&](int t, int r) { return s * kStep + 16 * (lane >> 4) + 4 * t + r; };
-      probabilities<M, NP, D, MT, MASKED>(sc, lim, key, a.scale, st, p);
+      const auto key = [](int t, int r) { return 4 * t + r; };
+      probabilities<M, NP, D, MT, MASKED>(sc, lim, s * kStep + 16 * (lane >> 4), key, a.scale, st, p);
       __builtin_amdgcn_sched_barrier(0);
       weigh<M, NP, D, MT, MASKED>(values, p, lim, s * kStep, b.limit, lane, st);
       load_values<D>(a, b, w, lane, values);
@@ -953,20 +969,21 @@ __device__ inline void note_nan(Raw4<D>& raw, int base, int limit, uint32_t* nan
     bool is_v;
     int x;
     if (!unit<D>(i, is_v, x) || !is_v) continue;
-    const int slice = x / (D / 2), pair = x % (D / 2);
+    const int slice = x / (D / 2), pair = x % (D / 2), left = limit - base - 16 * slice;
+    uint32_t bits = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       uint32_t sc = raw.scale[i][w];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const uint32_t sh = 8 * t;
-        const bool seen = base + 16 * slice + 4 * w + t < limit, bad = ((sc >> sh) & 255) == 255;
-        if (seen && bad && (pair & 15) == 0)
-          atomicOr(nan + (pair >> 4) * 2 + (slice >> 1), 1u << (16 * (slice & 1) + 4 * w + t));
+        const bool seen = 4 * w + t < left, bad = ((sc >> sh) & 255) == 255;
+        if (seen && bad) bits |= 1u << (4 * w + t);
         if (!seen || bad) sc = (sc & ~(255u << sh)) | 127u << sh;
       }
       raw.scale[i][w] = sc;
     }
+    if (bits && (pair & 15) == 0) atomicOr(nan + (pair >> 4) * 2 + (slice >> 1), bits << (16 * (slice & 1)));
   }
 }
 
@@ -1041,8 +1058,8 @@ __device__ inline void attend_lds(const char* lds, const u32x4 (&q)[Prompt4<D>::
     }
   }
   u32x4 p[MT][1][2];
-  const auto key = [&](int t, int r) { return base + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; };
-  probabilities<M, 1, D, MT, MASKED>(sc, sees, key, scale, st, p);
+  const auto key = [](int t, int r) { return 32 * (t >> 1) + 4 * (t & 1) + r; };
+  probabilities<M, 1, D, MT, MASKED>(sc, sees, base + 8 * g, key, scale, st, p);
   __builtin_amdgcn_sched_barrier(0);
   {
     u32x4 v[2][2];
@@ -1082,17 +1099,32 @@ __device__ inline void attend_lds(const char* lds, const u32x4 (&q)[Prompt4<D>::
   }
 }
 
-// The query block `flat` of the rows that take this kernel, in their order, counted
-// from the last one's last block: causal blocks' work grows along a row.
+// The query block `flat` of the rows that take this kernel: of each 64 rows the one
+// with the most keys first, and its last block first (causal blocks' work grows
+// along a row), so that the longest start first.
 template <int ROWS>
 __device__ inline bool flat_block(const Attn4Args& a, int head, int64_t flat, int& row, int& qb) {
   const int lane = threadIdx.x & 63;
-  const auto blocks = [&](int r) {
-    const int64_t n = r < a.num_rows ? static_cast<int64_t>(imin(a.q_lens[r], a.max_q)) * a.group : 0;
-    return n > kDirect ? (n + ROWS - 1) / ROWS : 0;
-  };
-  for (int r0 = (a.num_rows - 1) / 64 * 64; r0 >= 0; r0 -= 64) {
-    const int64_t mine = blocks(r0 + 63 - lane);  // the last row first
+  for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
+    int64_t mine = 0;
+    int keys = -1;
+    if (r0 + lane < a.num_rows) {
+      const int64_t n = static_cast<int64_t>(imin(a.q_lens[r0 + lane], a.max_q)) * a.group;
+      if (n > kDirect) {
+        mine = (n + ROWS - 1) / ROWS;
+        keys = a.k_lens[r0 + lane];
+      }
+    }
+    int rank = 0;  // rows that come before the lane's
+    for (uint64_t left = __ballot(mine > 0); left; left &= left - 1) {
+      const int other = __builtin_ctzll(left), k = __builtin_amdgcn_readlane(keys, other);
+      rank += k > keys || (k == keys && other < lane) ? 1 : 0;
+    }
+    // (lanes without blocks go behind the others, in their order)
+    const uint64_t with = __ballot(mine > 0);
+    if (mine == 0) rank = __popcll(with) + __popcll(~with & ((uint64_t{1} << lane) - 1));
+    const int from = __builtin_amdgcn_ds_permute(rank * 4, lane);  // the row of rank `lane`
+    mine = __shfl(mine, from, kWave);
     int64_t ends = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -1102,7 +1134,7 @@ __device__ inline bool flat_block(const Attn4Args& a, int head, int64_t flat, in
     const uint64_t after = __ballot(ends > flat);
     if (after) {
       const int at = __builtin_ctzll(after);
-      row = r0 + 63 - at;
+      row = r0 + __shfl(from, at, kWave);
       qb = static_cast<int>(__shfl(ends, at, kWave) - 1 - flat);
       row = __builtin_amdgcn_readfirstlane(row);
       qb = __builtin_amdgcn_readfirstlane(qb);
@@ -1257,6 +1289,60 @@ merge_4bit_kernel(Attn4Args a) {
   if (a.lse && lane == 0) a.lse[tok * a.l_st + hd * a.l_sh] = sum == 0 ? -INFINITY : (ref + F32::log2(sum)) * kLn2;
 }
 
+// NaN of the cache into the outputs of the queries that see it, where an attention
+// over finite copies of its values wrote them.  A work-group looks through
+// kNanRecords records of a row and kv head: their scales are a seventeenth of them.
+constexpr int kNanRecords = 64;
+
+struct Nan4Args {
+  Attn4Args a;
+  const int32_t* rows;  // rows of the block table
+};
+
+template <class IO>
+__global__ void __launch_bounds__(256)
+spread_nan_4bit_kernel(Nan4Args n, int d) {
+  const Attn4Args& a = n.a;
+  __shared__ int32_t first[9];  // first key with a NaN: in K, in each group of V
+  const int r = blockIdx.x / a.hkv, head = blockIdx.x % a.hkv;
+  const int row = n.rows[r];
+  const int64_t held = a.bt_stride * a.block_size;
+  int k_len = imin(imax(a.k_lens[r], 0), a.max_k);
+  if (k_len > held) k_len = static_cast<int>(held);
+  if (threadIdx.x < 9) first[threadIdx.x] = INT32_MAX;
+  __syncthreads();
+  const int begin = static_cast<int>(blockIdx.y) * kNanRecords, end = imin(begin + kNanRecords, (k_len + 15) / 16);
+  const int chunks = d / 16, groups = d / 32;  // 16-byte pieces: K's groups, then V's
+  for (int u = static_cast<int>(threadIdx.x); u < (end - begin) * chunks; u += 256) {
+    const int rec = begin + u / chunks, c = u % chunks;
+    const int id = imin(imax(a.bt[static_cast<int64_t>(row) * a.bt_stride + rec / a.spb], 0), a.num_blocks - 1);
+    const char* p = a.cache + id * a.block_stride +
+                    (static_cast<int64_t>(rec % a.spb) * a.hkv + head) * (17 * d) + 16 * d + c * 16;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+    for (int i = 0; i < 16; ++i) {
+      if (((x[i >> 2] >> (8 * (i & 3))) & 255) != 255) continue;
+      const int t = c < groups ? (i & 3) * 4 + (i >> 2) : i;
+      if (rec * 16 + t < k_len) atomicMin(&first[c < groups ? 0 : 1 + c - groups], rec * 16 + t);
+    }
+  }
+  __syncthreads();
+  int any = INT32_MAX;
+  for (int g = 0; g <= groups; ++g) any = imin(any, first[g]);
+  if (any == INT32_MAX) return;
+  const int n_q = imin(a.q_lens[r], a.max_q);
+  for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_q) * a.group; i += 256) {
+    const int64_t tok = a.q_starts[r] + i / a.group;
+    const int h = head * a.group + static_cast<int>(i % a.group);
+    const int64_t last = a.causal ? static_cast<int64_t>(a.q_offs[r]) + i / a.group : k_len - 1;
+    if (tok < 0 || tok >= a.total_query) continue;
+    typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + h * a.o_sh;
+    for (int g = 0; g < groups; ++g)
+      if (first[0] <= last || first[1 + g] <= last)
+        for (int e = 0; e < 32; ++e) o[32 * g + e] = IO::from_float(__builtin_nanf(""));
+    if (first[0] <= last && a.lse) a.lse[tok * a.l_st + h * a.l_sh] = __builtin_nanf("");
+  }
+}
+
 constexpr int64_t kWholeSteps = 128;
 
 // Split of a call's rows that take one of the two kernels: query blocks (of a row
@@ -1405,21 +1491,24 @@ extern "C" int kvhot_reshape_and_cache_4bit(
 
 extern "C" int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_bytes, const void* slots, int slot_is_int64,
                                      int64_t num_slots, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
-                                     int64_t num_blocks, void* key, void* value, int dtype, void* stream) {
+                                     int64_t num_blocks, void* key, void* value, int as_blocks, int dtype, void* stream) {
   clear_error();
   if (dtype_size(dtype) == 0) return set_error(KVHOT_EINVAL, "read_cache_4bit: bad dtype");
   if (num_slots < 0) return set_error(KVHOT_EINVAL, "read_cache_4bit: bad sizes");
   if (int e = check_pool("read_cache_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
     return e;
   if (num_slots == 0) return 0;
-  if (!key || !value || !slots) return set_error(KVHOT_EINVAL, "read_cache_4bit: null pointer");
+  if (!key || (!value && !as_blocks) || !slots) return set_error(KVHOT_EINVAL, "read_cache_4bit: null pointer");
+  if (as_blocks && num_slots % 16 != 0)
+    return set_error(KVHOT_EINVAL, "read_cache_4bit: blocks of slots that are no multiple of 16");
   if (reinterpret_cast<uintptr_t>(key) % 16 || reinterpret_cast<uintptr_t>(value) % 16)
     return set_error(KVHOT_EINVAL, "read_cache_4bit: misaligned tensors");
   const int64_t units = (num_slots + 15) / 16 * num_kv_heads * 2;
   if ((units + 3) / 4 > 0x7fffffff) return set_error(KVHOT_EUNSUPPORTED, "read_cache_4bit: too many slots");
   const Pool4 pool = pool_of(cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks);
 #define KVHOT_LAUNCH(T, S, D)                                                                                    \
-  hipLaunchKernelGGL((read_4bit_kernel<T, S, D>), dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,    \
+  hipLaunchKernelGGL((as_blocks ? read_4bit_kernel<T, S, D, true> : read_4bit_kernel<T, S, D, false>),              \
+                     dim3(static_cast<uint32_t>((units + 3) / 4)), dim3(256), 0,                                 \
                      static_cast<hipStream_t>(stream), pool, static_cast<const S*>(slots), num_slots, units,     \
                      static_cast<T::storage*>(key), static_cast<T::storage*>(value))
   KVHOT_FOR_TYPES(KVHOT_LAUNCH, KVHOT_FOR_DIMS)
@@ -1497,6 +1586,83 @@ int launch_4bit(const Plan4& p, Attn4Args& a, int64_t d, char* ws, hipStream_t s
 
 }  // namespace
 
+static Attn4Args args_4bit(const void* q, const int64_t* q_strides, const void* cache, int64_t block_stride_bytes, void* out,
+                           const int64_t* out_strides, float* lse, const int64_t* lse_strides, const int32_t* block_table,
+                           int64_t bt_row_stride, const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_starts,
+                           const int32_t* q_pos_offsets, int64_t num_rows, int64_t total_query, int64_t max_q_len,
+                           int64_t max_k_len, int64_t num_q_heads, int64_t num_kv_heads, int64_t block_size,
+                           int64_t num_blocks, float scale, int attn_flags, int dtype) {
+  const int64_t es = dtype_size(dtype);
+  Attn4Args a{};
+  a.q = q;
+  a.q_st = q ? q_strides[0] : 0;
+  a.q_sh = q ? q_strides[1] : 0;
+  a.cache = static_cast<const char*>(cache);
+  a.block_stride = block_stride_bytes;
+  a.out = out;
+  a.o_st = out_strides[0];
+  a.o_sh = out_strides[1];
+  a.lse = lse;
+  a.l_st = lse ? lse_strides[0] : 0;
+  a.l_sh = lse ? lse_strides[1] : 0;
+  a.bt = block_table;
+  a.bt_stride = bt_row_stride;
+  a.q_lens = q_lens;
+  a.k_lens = k_lens;
+  a.q_starts = q_starts;
+  a.q_offs = q_pos_offsets;
+  a.total_query = total_query;
+  a.num_rows = static_cast<int32_t>(num_rows);
+  a.hq = static_cast<int32_t>(num_q_heads);
+  a.hkv = static_cast<int32_t>(num_kv_heads);
+  a.group = a.hq / a.hkv;
+  a.block_size = static_cast<int32_t>(block_size);
+  a.num_blocks = static_cast<int32_t>(num_blocks);
+  a.causal = attn_flags & KVHOT_CAUSAL;
+  a.scale = std::fabs(scale) * kLog2e;
+  a.negate = scale < 0;
+  a.q_vec = aligned(q, es, 16, {a.q_st, a.q_sh});
+  a.max_q = static_cast<int32_t>(max_q_len);
+  a.max_k = static_cast<int32_t>(max_k_len);
+  a.spb = a.block_size / 16;
+  return a;
+}
+
+extern "C" int kvhot_spread_nan_4bit(const void* cache, int64_t block_stride_bytes, void* out, const int64_t out_strides[3],
+                                     float* lse, const int64_t lse_strides[2], const int32_t* block_table,
+                                     int64_t bt_row_stride, const int32_t* rows, const int32_t* q_lens,
+                                     const int32_t* k_lens, const int32_t* q_starts, const int32_t* q_pos_offsets,
+                                     int64_t num_rows, int64_t total_query, int64_t max_q_len, int64_t max_k_len,
+                                     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size,
+                                     int64_t num_blocks, int attn_flags, int dtype, void* stream) {
+  clear_error();
+  if (int e = check_attention(num_rows, total_query, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
+    return e;
+  if (int e = check_pool("spread_nan_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
+    return e;
+  if (attn_flags & ~KVHOT_CAUSAL) return set_error(KVHOT_EINVAL, "spread_nan_4bit: unknown attn_flags");
+  if (num_rows == 0 || total_query == 0 || max_q_len == 0 || max_k_len == 0 || num_blocks == 0) return 0;
+  if (!out || !out_strides || (lse && !lse_strides) || !block_table || !rows || !q_lens || !k_lens || !q_starts || !q_pos_offsets)
+    return set_error(KVHOT_EINVAL, "spread_nan_4bit: null pointer");
+  if (out_strides[2] != 1 || bt_row_stride <= 0) return set_error(KVHOT_EINVAL, "spread_nan_4bit: bad strides");
+  const int64_t y = ((max_k_len + 15) / 16 + kNanRecords - 1) / kNanRecords;
+  if (num_rows * num_kv_heads > 0x7fffffff || y > 65535)
+    return set_error(KVHOT_EUNSUPPORTED, "spread_nan_4bit: too many work-groups");
+  Nan4Args n{args_4bit(nullptr, nullptr, cache, block_stride_bytes, out, out_strides, lse, lse_strides, block_table,
+                       bt_row_stride, q_lens, k_lens, q_starts, q_pos_offsets, num_rows, total_query, max_q_len, max_k_len,
+                       num_q_heads, num_kv_heads, block_size, num_blocks, 1.0f, attn_flags, dtype),
+             rows};
+  const dim3 grid(static_cast<uint32_t>(num_rows * num_kv_heads), static_cast<uint32_t>(y));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int d = static_cast<int>(head_dim);
+  switch (dtype) {
+    case KVHOT_F32: hipLaunchKernelGGL(spread_nan_4bit_kernel<F32>, grid, dim3(256), 0, s, n, d); break;
+    case KVHOT_F16: hipLaunchKernelGGL(spread_nan_4bit_kernel<F16>, grid, dim3(256), 0, s, n, d); break;
+    default: hipLaunchKernelGGL(spread_nan_4bit_kernel<BF16>, grid, dim3(256), 0, s, n, d); break;
+  }
+  return launch_status("spread_nan_4bit");
+}
+
 extern "C" int kvhot_paged_attention_4bit(
     const void* q, const int64_t q_strides[3], const void* cache, int64_t block_stride_bytes, void* out,
     const int64_t out_strides[3], float* lse, const int64_t lse_strides[2], const int32_t* block_table,
@@ -1523,40 +1689,9 @@ extern "C" int kvhot_paged_attention_4bit(
   const int64_t need = plan.direct.ws_bytes + plan.prompt.ws_bytes;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(KVHOT_EWORKSPACE, "paged_attention_4bit: workspace missing or too small");
-  const int64_t es = dtype_size(dtype);
-  Attn4Args a;
-  a.q = q;
-  a.q_st = q_strides[0];
-  a.q_sh = q_strides[1];
-  a.cache = static_cast<const char*>(cache);
-  a.block_stride = block_stride_bytes;
-  a.out = out;
-  a.o_st = out_strides[0];
-  a.o_sh = out_strides[1];
-  a.lse = lse;
-  a.l_st = lse ? lse_strides[0] : 0;
-  a.l_sh = lse ? lse_strides[1] : 0;
-  a.bt = block_table;
-  a.bt_stride = bt_row_stride;
-  a.q_lens = q_lens;
-  a.k_lens = k_lens;
-  a.q_starts = q_starts;
-  a.q_offs = q_pos_offsets;
-  a.total_query = total_query;
-  a.num_rows = static_cast<int32_t>(num_rows);
-  a.hq = static_cast<int32_t>(num_q_heads);
-  a.hkv = static_cast<int32_t>(num_kv_heads);
-  a.group = a.hq / a.hkv;
-  a.block_size = static_cast<int32_t>(block_size);
-  a.num_blocks = static_cast<int32_t>(num_blocks);
-  a.causal = attn_flags & KVHOT_CAUSAL;
-  a.scale = std::fabs(scale) * kLog2e;
-  a.negate = scale < 0;
-  a.q_vec = aligned(q, es, 16, {q_strides[0], q_strides[1]});
-  a.o_vec = aligned(out, es, 16, {out_strides[0], out_strides[1]});
-  a.max_q = static_cast<int32_t>(max_q_len);
-  a.max_k = static_cast<int32_t>(max_k_len);
-  a.spb = a.block_size / 16;
+  Attn4Args a = args_4bit(q, q_strides, cache, block_stride_bytes, out, out_strides, lse, lse_strides, block_table,
+                          bt_row_stride, q_lens, k_lens, q_starts, q_pos_offsets, num_rows, total_query, max_q_len, max_k_len,
+                          num_q_heads, num_kv_heads, block_size, num_blocks, scale, attn_flags, dtype);
   a.direct = plan.limit;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {

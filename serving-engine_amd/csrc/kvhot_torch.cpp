@@ -416,19 +416,21 @@ PyObject* py_read4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = c10::hip::getCurrentHIPStream(p.pool.get_device()).stream();
     const int status = without_gil([&] {
       return g_read4(p.base(), p.pool.stride(1), slots.data_ptr(), is_long(slots), slots.size(0), p.heads(), p.dim,
-                     p.block_size(), p.pool.size(1), key.data_ptr(), value.data_ptr(), static_cast<int>(dtype), stream);
+                     p.block_size(), p.pool.size(1), key.data_ptr(), value.data_ptr(), 0, static_cast<int>(dtype), stream);
     });
     if (status != 0) return nullptr;
     return pair_of(key, value);
   });
 }
 
-// attention4(q, blocks, metadata, hq, hkv, scale, causal, workspaces) -> (o, l) | None
+// attention4(q, blocks, metadata, hq, hkv, scale, causal, workspaces, prompt_pairs) -> (o, l) | None
+//   (None where the host knows of a row that may have that many (query, head) pairs
+//   a kv head: prompts are planned in Python.)
 PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return or_none([&]() -> PyObject* {
     Tensor q, kv, q_lens, k_lens, q_starts, q_offs, bt, ws;
-    int64_t hq, hkv, max_q, max_k, bt_stride;
-    if (n != 8 || !g_attention4 || !g_workspace_bytes4 || !gpu_tensor(a[0], q) || !gpu_tensor(a[1], kv) ||
+    int64_t hq, hkv, max_q, max_k, bt_stride, prompt;
+    if (n != 9 || !as_int(a[8], prompt) || !g_attention4 || !g_workspace_bytes4 || !gpu_tensor(a[0], q) || !gpu_tensor(a[1], kv) ||
         !PyDict_CheckExact(a[2]) || !as_int(a[3], hq) || !as_int(a[4], hkv) || !PyFloat_Check(a[5]) || !PyBool_Check(a[6]) ||
         !PyDict_CheckExact(a[7]))
       return nullptr;
@@ -448,6 +450,8 @@ PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !as_int(PyDict_GetItemWithError(meta, g_names.max_q_len), max_q) ||
         !as_int(PyDict_GetItemWithError(meta, g_names.max_k_len), max_k))
       return nullptr;
+    PyObject* host = PyDict_GetItemWithError(meta, g_names.host_q_lens);
+    if (host && host != Py_None && max_q * (hq / hkv) >= prompt) return nullptr;
     const int64_t need = g_workspace_bytes4(rows, q.size(0), max_q, max_k, hq, hkv, q.size(2), dt);
     void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
     if (need < 0 || (need > 0 && !stream_workspace(a[7], d, stream, need, ws))) return nullptr;

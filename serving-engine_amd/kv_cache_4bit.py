@@ -12,11 +12,12 @@ The reference caches in the model's dtype only
 """
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 from . import _lib
 from .block import BLOCK_SIZE
-from .paged_attention_kernel import _WORKSPACES, _check_meta, _host_max, _workspace
+from .paged_attention_kernel import _WORKSPACES, _attend_into, _check_meta, _host_max, _order_list, _workspace
 
 HEAD_DIMS_4BIT = (64, 96, 128, 256)
 RECORD_TOKENS = 16  # tokens of a record; a block holds block_size / 16 of them a kv head
@@ -147,7 +148,7 @@ class _PagedKVCache4Bit:
                 status = _lib.load().kvhot_read_cache_4bit(
                     base, kv.stride(1), read_index.data_ptr(), 1 if read_index.dtype is torch.int64 else 0, n,
                     self.num_kv_heads, self.head_dim, self.block_size, self.num_blocks, key.data_ptr(),
-                    value.data_ptr(), _lib.dtype_code(self.dtype), _lib.stream_handle(kv.device))
+                    value.data_ptr(), 0, _lib.dtype_code(self.dtype), _lib.stream_handle(kv.device))
             _lib.check(status, "kvhot_read_cache_4bit")
         return key, value
 
@@ -192,7 +193,8 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     cache reaches the queries that see it and no other; in fp16, cached values beyond
     its range (of a pool written from another dtype) are infinite.
     """
-    out = _lib.native().attention4(q, kv_blocks, metadata, num_q_heads, num_kv_heads, scale, bool(is_causal), _WORKSPACES)
+    out = _lib.native().attention4(q, kv_blocks, metadata, num_q_heads, num_kv_heads, scale, bool(is_causal), _WORKSPACES,
+                                   PROMPT_PAIRS)
     if out is not None:
         return out
     if q.dim() != 3:
@@ -209,7 +211,7 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     device = q.device
     if device.type != "cuda" or kv_blocks.device != device:
         raise ValueError("q and kv_blocks must be on the same GPU")
-    dtype = _lib.dtype_code(q.dtype)
+    _lib.dtype_code(q.dtype)
     q_lens = metadata["q_lens"]
     num_rows = q_lens.shape[0]
     o = torch.empty_like(q)
@@ -223,21 +225,135 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     bt_stride = int(metadata.get("block_table_row_stride", bt.shape[1] if bt.dim() == 2 else 0))
     max_q = _host_max(metadata, "max_q_len", "q_lens")
     max_k = _host_max(metadata, "max_k_len", "k_lens")
-    lib = _lib.load()
-    stream = _lib.stream_handle(device)
-    need = lib.kvhot_paged_attention_4bit_workspace_bytes(num_rows, total_query, max_q, max_k, num_q_heads, num_kv_heads,
-                                                          head_dim, dtype)
+    plan = _prompts(metadata, device, num_q_heads // num_kv_heads, spb * RECORD_TOKENS)
+    with torch.cuda.device(device):
+        if plan is None:
+            _attend(q, kv_blocks, metadata, q_lens, max_q, max_k, bt_stride, scale, is_causal, o, l)
+        else:
+            if plan.max_q:
+                _attend(q, kv_blocks, metadata, plan.q_lens, plan.max_q, plan.max_k, bt_stride, scale, is_causal, o, l)
+            _attend_prompts(q, kv_blocks, metadata, plan, bt_stride, scale, is_causal, o, l)
+    return o, l
+
+
+def _attend(q, kv_blocks, metadata, q_lens, max_q, max_k, bt_stride, scale, is_causal, o, l):
+    """kvhot_paged_attention_4bit of the rows that have queries in q_lens."""
+    lib, device = _lib.load(), q.device
+    total_query, hq, head_dim = q.shape
+    num_blocks, spb, hkv, _ = kv_blocks.shape
+    num_rows, dtype, stream = q_lens.shape[0], _lib.dtype_code(q.dtype), _lib.stream_handle(device)
+    need = lib.kvhot_paged_attention_4bit_workspace_bytes(num_rows, total_query, max_q, max_k, hq, hkv, head_dim, dtype)
     if need < 0:
         _lib.check(int(need), "kvhot_paged_attention_4bit_workspace_bytes")
     ws = _workspace(device, stream, need)
-    with torch.cuda.device(device):
-        status = lib.kvhot_paged_attention_4bit(
-            q.data_ptr(), _lib.i64_array(q.stride()), kv_blocks.data_ptr(), kv_blocks.stride(0),
-            o.data_ptr(), _lib.i64_array(o.stride()), l.data_ptr(), _lib.i64_array(l.stride()),
-            bt.data_ptr(), bt_stride, q_lens.data_ptr(), metadata["k_lens"].data_ptr(),
-            metadata["q_starts"].data_ptr(), metadata["q_pos_offsets"].data_ptr(),
-            num_rows, total_query, max_q, max_k, num_q_heads, num_kv_heads, head_dim, spb * RECORD_TOKENS, num_blocks,
-            float(scale), _lib.KVHOT_CAUSAL if is_causal else 0, dtype,
-            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream)
+    status = lib.kvhot_paged_attention_4bit(
+        q.data_ptr(), _lib.i64_array(q.stride()), kv_blocks.data_ptr(), kv_blocks.stride(0),
+        o.data_ptr(), _lib.i64_array(o.stride()), l.data_ptr(), _lib.i64_array(l.stride()),
+        metadata["block_table"].data_ptr(), bt_stride, q_lens.data_ptr(), metadata["k_lens"].data_ptr(),
+        metadata["q_starts"].data_ptr(), metadata["q_pos_offsets"].data_ptr(),
+        num_rows, total_query, max_q, max_k, hq, hkv, head_dim, spb * RECORD_TOKENS, num_blocks,
+        float(scale), _lib.KVHOT_CAUSAL if is_causal else 0, dtype,
+        ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream)
     _lib.check(status, "kvhot_paged_attention_4bit")
-    return o, l
+
+
+class _Prompts:
+    """What a step's calls know of its prompts (rows of at least PROMPT_PAIRS
+    (query, head) pairs a kv head), planned once: ``meta``, the metadata of those
+    rows alone over a pool of their own keys' copies, block after block; ``slots``
+    [16 * blocks], where those keys are (-1 behind a row's end); ``rows``, their
+    rows in the step's block table; ``q_lens``, the step's with theirs 0, and the
+    bounds of the rows that are left."""
+
+
+# (query, head) pairs a kv head from which a row is attended over dense copies.
+PROMPT_PAIRS = 512
+# Bytes that a call's copies may take.
+PROMPT_BYTES = 8 << 30
+
+
+def _prompts(metadata, device, group, block_size):
+    """The step's _Prompts, planned from the host copies of its lengths and kept in
+    the metadata; None without host copies or prompts."""
+    host_q = metadata.get("host_q_lens")
+    if host_q is None or _host_max(metadata, "max_q_len", "q_lens") * group < PROMPT_PAIRS:
+        return None
+    key = ("prompts4", group, block_size, str(device))
+    cache = metadata.setdefault("_schedules", {})
+    if key in cache:
+        hit = cache[key]
+        _order_list(metadata, key, hit, device)
+        return None if hit is None else hit[1]
+    if torch.cuda.is_current_stream_capturing():
+        return None  # (as _schedule: a copy from here would be replayed)
+    host_k, host_off = metadata["host_k_lens"], metadata["host_q_pos_offsets"]
+    rows = np.flatnonzero((host_q.astype(np.int64) * group >= PROMPT_PAIRS) & (host_k > 0))
+    if not rows.size:
+        cache[key] = None
+        return None
+    r, n = len(host_q), len(rows)
+    k_lens = host_k[rows].astype(np.int64)
+    blocks = -(-k_lens // BLOCK_SIZE)
+    ends = np.cumsum(blocks)
+    total, width = int(ends[-1]), int(blocks.max())
+    table = np.zeros((n, width), dtype=np.int32)
+    slots = np.full((total, BLOCK_SIZE), -1, dtype=np.int64)
+    for i, row in enumerate(rows):
+        first = int(ends[i] - blocks[i])
+        table[i, :blocks[i]] = np.arange(first, ends[i])
+        j = np.arange(k_lens[i])
+        slots[first:ends[i]].reshape(-1)[:k_lens[i]] = (
+            metadata["host_block_table"][row, j // block_size].astype(np.int64) * block_size + j % block_size)
+    short = host_q.copy()
+    short[rows] = 0
+    left = np.flatnonzero(short > 0)
+    per_row = [metadata["host_" + x][rows].astype(np.int32) for x in ("q_lens", "k_lens", "q_starts", "q_pos_offsets")]
+    ints = [short.astype(np.int32), *per_row, rows.astype(np.int32), table.reshape(-1)]
+    at = np.cumsum([0] + [x.size for x in ints])
+    pad = int(at[-1]) % 2  # the slots are 8-byte values
+    staged = torch.empty(int(at[-1]) + pad + 2 * slots.size, dtype=torch.int32, pin_memory=True)
+    staged.numpy()[:at[-1]] = np.concatenate(ints)
+    staged.numpy()[at[-1] + pad:] = slots.reshape(-1).view(np.int32)
+    buf = staged.to(device, non_blocking=True)
+    dev = [buf[a:b] for a, b in zip(at[:-1], at[1:])]
+    p = _Prompts()
+    p.q_lens, p.rows, p.slots = dev[0], dev[5], buf[at[-1] + pad:].view(torch.int64)
+    p.blocks = total
+    p.max_q = int(short.max()) if left.size else 0
+    p.max_k = int(host_k[left].max()) if left.size else 0
+    p.meta = dict(zip(("q_lens", "k_lens", "q_starts", "q_pos_offsets"), dev[1:5]))
+    p.meta.update(zip(("host_q_lens", "host_k_lens", "host_q_starts", "host_q_pos_offsets"), per_row))
+    p.meta.update(block_table=dev[6].view(n, width), host_block_table=table, block_table_row_stride=width,
+                  max_q_len=int(per_row[0].max()), max_k_len=int(k_lens.max()))
+    stream = torch.cuda.current_stream(device)
+    event = torch.cuda.Event()
+    event.record(stream)
+    metadata.setdefault("_schedule_streams", {})[key] = (event, {stream.cuda_stream})
+    cache[key] = (buf, p)
+    return p
+
+
+def _attend_prompts(q, kv_blocks, metadata, p, bt_stride, scale, is_causal, o, l):
+    """The prompts' attention: their keys as dense copies, once for all their
+    queries, then the 16- and 32-bit pools' attention over those, then the NaN
+    that the copies left out."""
+    lib, device, dtype = _lib.load(), q.device, _lib.dtype_code(q.dtype)
+    num_blocks, spb, hkv, rec = kv_blocks.shape
+    total_query, hq, d = q.shape
+    stream = _lib.stream_handle(device)
+    flags = _lib.KVHOT_CAUSAL if is_causal else 0
+    pool = torch.empty(p.blocks, hkv, 2, BLOCK_SIZE, d, dtype=q.dtype, device=device)
+    k, v = pool.permute(2, 0, 3, 1, 4)  # [blocks, tokens, Hkv, D] each, kv-interleaved
+    status = lib.kvhot_read_cache_4bit(
+        kv_blocks.data_ptr(), kv_blocks.stride(0), p.slots.data_ptr(), 1, p.blocks * BLOCK_SIZE, hkv, d,
+        spb * RECORD_TOKENS, num_blocks, pool.data_ptr(), None, 1, dtype, stream)
+    _lib.check(status, "kvhot_read_cache_4bit")
+    _attend_into(q, k, v, p.meta, hq, hkv, scale, is_causal, 0, flags, o, l)
+    m = p.meta
+    status = lib.kvhot_spread_nan_4bit(
+        kv_blocks.data_ptr(), kv_blocks.stride(0), o.data_ptr(), _lib.i64_array(o.stride()), l.data_ptr(),
+        _lib.i64_array(l.stride()), metadata["block_table"].data_ptr(), bt_stride, p.rows.data_ptr(),
+        m["q_lens"].data_ptr(), m["k_lens"].data_ptr(), m["q_starts"].data_ptr(), m["q_pos_offsets"].data_ptr(),
+        p.rows.shape[0], total_query, m["max_q_len"], m["max_k_len"], hq, hkv, d, spb * RECORD_TOKENS, num_blocks, flags,
+        dtype, stream)
+    _lib.check(status, "kvhot_spread_nan_4bit")

@@ -230,7 +230,7 @@ def paged_flash_attention(q, k_cache, v_cache, metadata, num_q_heads, num_kv_hea
     device = q.device
     if device.type != "cuda" or k_cache.device != device or v_cache.device != device:
         raise ValueError("q, k_cache and v_cache must be on the same GPU")
-    dtype = _lib.dtype_code(q.dtype)
+    _lib.dtype_code(q.dtype)
 
     q_lens = metadata["q_lens"]
     num_rows = q_lens.shape[0]
@@ -238,6 +238,17 @@ def paged_flash_attention(q, k_cache, v_cache, metadata, num_q_heads, num_kv_hea
     l = torch.empty((total_query, num_q_heads), dtype=torch.float32, device=device)
     if num_rows == 0 or total_query == 0:
         return o, l
+    _attend_into(q, k_cache, v_cache, metadata, num_q_heads, num_kv_heads, scale, is_causal, pt, flags, o, l)
+    return o, l
+
+
+def _attend_into(q, k_cache, v_cache, metadata, num_q_heads, num_kv_heads, scale, is_causal, pt, flags, o, l):
+    """The attention of paged_flash_attention's checked arguments into o and l."""
+    device, dtype = q.device, _lib.dtype_code(q.dtype)
+    total_query, _, head_dim = q.shape
+    num_blocks, block_size = k_cache.shape[:2]
+    num_rows = metadata["q_lens"].shape[0]
+    q_lens = metadata["q_lens"]
     for name in ("q_lens", "k_lens", "q_starts", "q_pos_offsets"):
         _check_meta(name, metadata[name], device, num_rows)
     bt = metadata["block_table"]
@@ -276,7 +287,6 @@ def paged_flash_attention(q, k_cache, v_cache, metadata, num_q_heads, num_kv_hea
         ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
         stream)
     _lib.check(status, "kvhot_paged_attention")
-    return o, l
 
 
 def build_paged_batch_metadata(scheduler_output, device="cuda", num_blocks=None):

@@ -55,7 +55,7 @@ def test_the_same_bits(cuda, sea, monkeypatch):
 def test_other_calls_are_left_alone(cuda, sea):
     n = sea_module("_lib").native()
     for f in (n.append4, n.read4, n.attention4, n.norm_rope, n.tables):
-        assert f() is None and f(*[None] * 5) is None and f(*[None] * 7) is None and f(*[None] * 8) is None
+        assert f() is None and f(*[None] * 5) is None and f(*[None] * 7) is None and f(*[None] * 8) is None and f(*[None] * 9) is None
     cache = sea._PagedKVCache4Bit(sea.allocate_kv_cache_4bit(1, 3, 2, 64), 64)
     k, slots = torch.zeros(1, 2, 4, 64, device=cuda, dtype=BF16), torch.arange(4, device=cuda)
     pool, code = cache.kv_cache, cache._code

@@ -57,7 +57,7 @@ def test_append_refusals(lib, kw, code):
 def test_calls_without_work_are_taken(lib):
     assert lib.kvhot_reshape_and_cache_4bit(*append_args(tokens=0, key=None)) == 0
     assert lib.kvhot_reshape_and_cache_4bit(*append_args(blocks=0, cache=None)) == 0
-    assert lib.kvhot_read_cache_4bit(P, 4 * 17 * 128, None, 1, 0, 4, 128, 16, 10, None, None, 2, None) == 0
+    assert lib.kvhot_read_cache_4bit(P, 4 * 17 * 128, None, 1, 0, 4, 128, 16, 10, None, None, 0, 2, None) == 0
     assert lib.kvhot_paged_attention_4bit(*attention_args(rows=0)) == 0
     assert lib.kvhot_paged_attention_4bit(*attention_args(total=0)) == 0
     assert lib.kvhot_norm_rope(*rope_args(tokens=0)) == 0
@@ -65,10 +65,10 @@ def test_calls_without_work_are_taken(lib):
 
 @pytest.mark.parametrize("kw,code", [
     (dict(slots=None), EINVAL), (dict(key=None), EINVAL), (dict(key=P + 4), EINVAL), (dict(n=-1), EINVAL),
-    (dict(d=32), EUNSUPPORTED), (dict(dtype=5), EINVAL),
+    (dict(d=32), EUNSUPPORTED), (dict(dtype=5), EINVAL), (dict(value=None), EINVAL), (dict(blocks_too=1), EINVAL),
 ])
 def test_read_refusals(lib, kw, code):
-    a = dict(cache=P, block=4 * 17 * 128, slots=P, i64=1, n=5, heads=4, d=128, bs=16, blocks=10, key=P, value=P, dtype=2, s=None)
+    a = dict(cache=P, block=4 * 17 * 128, slots=P, i64=1, n=5, heads=4, d=128, bs=16, blocks=10, key=P, value=P, blocks_too=0, dtype=2, s=None)
     a.update(kw)
     assert lib.kvhot_read_cache_4bit(*a.values()) == code
 
