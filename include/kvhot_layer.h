@@ -118,14 +118,15 @@ int kvhot_read_cache_4bit(const void* cache, int64_t block_stride_bytes,
  * and results (out in q's dtype, lse natural-log fp32, both for every query of
  * every row; a query with no visible key gets out = 0 and lse = -inf), with
  * the cache's values entering as what they stand for.  attn_flags: KVHOT_CAUSAL or
- * 0.  max_q_len / max_k_len must bound q_lens / k_lens.  The workspace holds
+ * 0.  max_q_len / max_k_len must bound q_lens / k_lens, sum_q_lens their sum
+ * (total_query does; a closer bound launches fewer empty work-groups).  The workspace holds
  * the partials of key ranges cut across work-groups and needs no clearing;
  * calls that share one must be ordered on one stream.
  * A NaN in the cache reaches the queries that see it and no other.  Repeated calls give the
  * same bits.
  */
 int64_t kvhot_paged_attention_4bit_workspace_bytes(
-    int64_t num_rows, int64_t total_query, int64_t max_q_len,
+    int64_t num_rows, int64_t sum_q_lens, int64_t max_q_len,
     int64_t max_k_len, int64_t num_q_heads, int64_t num_kv_heads,
     int64_t head_dim, int dtype);
 int kvhot_paged_attention_4bit(
@@ -134,10 +135,10 @@ int kvhot_paged_attention_4bit(
     float* lse, const int64_t lse_strides[2], const int32_t* block_table,
     int64_t bt_row_stride, const int32_t* q_lens, const int32_t* k_lens,
     const int32_t* q_starts, const int32_t* q_pos_offsets, int64_t num_rows,
-    int64_t total_query, int64_t max_q_len, int64_t max_k_len,
-    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
-    int64_t block_size, int64_t num_blocks, float scale, int attn_flags,
-    int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+    int64_t total_query, int64_t sum_q_lens, int64_t max_q_len,
+    int64_t max_k_len, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t block_size, int64_t num_blocks, float scale,
+    int attn_flags, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * For prompts that are attended over dense copies of their keys

@@ -110,7 +110,7 @@ LAYER_SIGNATURES = {
     ),
     "kvhot_paged_attention_4bit": (
         _int,
-        [_vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+        [_vp, _i64p, _vp, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
          _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _int, _int, _vp, _i64, _vp],
     ),
     "kvhot_spread_nan_4bit": (

@@ -31,15 +31,6 @@
 #include <initializer_list>
 #include <type_traits>
 
-#ifndef KVHOT_W4
-#define KVHOT_W4 3
-#endif
-#ifndef KVHOT_DIRECT
-#define KVHOT_DIRECT 16
-#endif
-#ifndef KVHOT_PW
-#define KVHOT_PW 8
-#endif
 
 namespace kvhot {
 
@@ -334,10 +325,8 @@ struct Attn4Args {
   float scale;     // |scale| * log2(e)
   int32_t negate;  // the scale is negative: Q's sign is turned
   int32_t q_vec;
-  // the padded grid
-  int32_t q_blocks, parts, part_steps, max_q, max_k, spb;
-  int64_t blocks;  // query blocks of the grid
-  int64_t direct;  // rows of more m-rows are the prompts' kernel's
+  // the grid
+  int32_t flat, parts, part_steps, max_q, max_k, spb;
   float* ws_o;
   float* ws_lse;
 };
@@ -354,7 +343,6 @@ struct Block4 {
   int32_t k_len;
   int32_t limit;             // keys that any of the m-rows sees
   int32_t least;             // keys that all of them see
-  int64_t all;               // m-rows of the row
 };
 
 __device__ inline int imin(int a, int b) { return a < b ? a : b; }
@@ -373,9 +361,9 @@ __device__ inline bool block_of(const Attn4Args& a, int row, int head, int qb, B
   b.head = head;
   const int n_q = imin(a.q_lens[row], a.max_q);
   b.first = qb * ROWS;
-  b.all = static_cast<int64_t>(n_q) * a.group;
-  if (n_q <= 0 || b.first >= b.all) return false;
-  b.rows = static_cast<int>(b.all - b.first < ROWS ? b.all - b.first : ROWS);
+  const int64_t all = static_cast<int64_t>(n_q) * a.group;
+  if (n_q <= 0 || b.first >= all) return false;
+  b.rows = static_cast<int>(all - b.first < ROWS ? all - b.first : ROWS);
   b.q0 = a.q_starts[row];
   b.off = a.q_offs[row];
   b.k_len = imin(imax(a.k_lens[row], 0), a.max_k);
@@ -488,17 +476,16 @@ __device__ inline void split_pair(float a, float b, uint32_t (&p)[NP]) {
   }
 }
 
-// Q^T of m-rows first .. first + 16 * MT of the block, as B operands: lane (n, g) has
-// elements 8 (NJ * g + j) on of m-row n (or 8 (4 j + g) on where the kernel reads K
-// that way), and how many keys it sees.
-template <class IO, class M, int NP, int D, int MT, bool STRIPED>
-__device__ inline void load_queries(const Attn4Args& a, const Block4& b, int first, int lane, u32x4 (&q)[MT][NP][D / 32],
+// Q^T of the block, as B operands: lane (n, g) has elements 8 (NJ * g + j) on of m-row
+// n of each tile; and how many keys that sees.
+template <class IO, class M, int NP, int D, int MT>
+__device__ inline void load_queries(const Attn4Args& a, const Block4& b, int lane, u32x4 (&q)[MT][NP][D / 32],
                                     int (&lim)[MT]) {
   constexpr int NJ = D / 32;
   const int n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int at = first + 16 * m + n, mr = b.first + at;
+    const int at = 16 * m + n, mr = b.first + at;
     const bool there = at < b.rows;
     const int tok = b.q0 + mr / a.group;
     lim[m] = there ? sees(a, b, mr) : b.limit;
@@ -509,7 +496,7 @@ __device__ inline void load_queries(const Attn4Args& a, const Block4& b, int fir
     for (int j = 0; j < NJ; ++j) {
       float x[8];
       if (ok) {
-        load8<IO>(src + 8 * (STRIPED ? 4 * j + g : NJ * g + j), a.q_vec, x);
+        load8<IO>(src + 8 * (NJ * g + j), a.q_vec, x);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = 0;
@@ -541,18 +528,18 @@ __device__ inline void clear(State4<D, MT>& st) {
   }
 }
 
-// Writes a wave's m-rows: to the outputs, or, of a block cut into parts, to the
-// workspace (rows from w0 on).  Register r of O^T's tile c is element(c, r).
-template <class IO, int D, int MT, class E>
-__device__ inline void finish(const Attn4Args& a, const Block4& b, int first, bool whole, int64_t w0, int lane,
-                              const State4<D, MT>& st, E element) {
+// Writes the block's m-rows: to the outputs, or, of a block cut into parts, to the
+// workspace (rows from w0 on).
+template <class IO, int D, int MT>
+__device__ inline void finish(const Attn4Args& a, const Block4& b, bool whole, int64_t w0, int lane,
+                              const State4<D, MT>& st) {
   const int n = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     float sum = st.sum[m];
     sum += __shfl_xor(sum, 16, kWave);
     sum += __shfl_xor(sum, 32, kWave);
-    const int at = first + 16 * m + n, mr = b.first + at;
+    const int at = 16 * m + n, mr = b.first + at;
     if (at >= b.rows) continue;
     const float inv = sum == 0 ? 0.0f : 1.0f / sum;  // no key seen: 0
     const float lse2 = sum == 0 ? -INFINITY : st.ref[m] + F32::log2(sum);
@@ -563,14 +550,14 @@ __device__ inline void finish(const Attn4Args& a, const Block4& b, int first, bo
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) o[element(c, r)] = IO::from_float(st.o[m][c][r] * inv);
+        for (int c = 0; c < D / 16; ++c) o[2 * pair_of<D>(4 * g + r, c >> 1) + (c & 1)] = IO::from_float(st.o[m][c][r] * inv);
       if (a.lse && g == 0) a.lse[tok * a.l_st + hd * a.l_sh] = lse2 * kLn2;
     } else {
       float* o = a.ws_o + (w0 + at) * D;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int c = 0; c < D / 16; ++c) o[element(c, r)] = st.o[m][c][r] * inv;
+        for (int c = 0; c < D / 16; ++c) o[2 * pair_of<D>(4 * g + r, c >> 1) + (c & 1)] = st.o[m][c][r] * inv;
       if (g == 0) a.ws_lse[w0 + at] = lse2;
     }
   }
@@ -799,8 +786,64 @@ __device__ inline void park(const State4<D, MT>& a, float* lds, int lane) {
 template <int D, int MT>
 constexpr int parked() { return MT * (D / 16 * 4 + 3) * kWave; }
 
+// The query block `flat` of all rows: of each 64 rows the one with the most keys
+// first, and its last block first (causal blocks' work grows along a row), so that
+// the longest start first.  (A grid of rows times the longest row's blocks would
+// launch work-groups for blocks that are not there, at 8 ns each.)
+template <int ROWS>
+__device__ inline bool flat_block(const Attn4Args& a, int64_t flat, int& row, int& qb) {
+  const int lane = threadIdx.x & 63;
+  for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
+    int64_t mine = 0;
+    int keys = -1;
+    if (r0 + lane < a.num_rows) {
+      const int64_t n = static_cast<int64_t>(imin(a.q_lens[r0 + lane], a.max_q)) * a.group;
+      if (n > 0) {
+        mine = (n + ROWS - 1) / ROWS;
+        keys = a.k_lens[r0 + lane];
+      }
+    }
+    int rank = 0;  // rows that come before the lane's
+    for (uint64_t left = __ballot(mine > 0); left; left &= left - 1) {
+      const int other = __builtin_ctzll(left), k = __builtin_amdgcn_readlane(keys, other);
+      rank += k > keys || (k == keys && other < lane) ? 1 : 0;
+    }
+    // (lanes without blocks go behind the others, in their order)
+    const uint64_t with = __ballot(mine > 0);
+    if (mine == 0) rank = __popcll(with) + __popcll(~with & ((uint64_t{1} << lane) - 1));
+    const int from = __builtin_amdgcn_ds_permute(rank * 4, lane);  // the row of rank `lane`
+    mine = __shfl(mine, from, kWave);
+    int64_t ends = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(ends, o, kWave);
+      if (lane >= o) ends += x;
+    }
+    const uint64_t after = __ballot(ends > flat);
+    if (after) {
+      const int at = __builtin_ctzll(after);
+      row = r0 + __shfl(from, at, kWave);
+      qb = static_cast<int>(__shfl(ends, at, kWave) - 1 - flat);
+      row = __builtin_amdgcn_readfirstlane(row);
+      qb = __builtin_amdgcn_readfirstlane(qb);
+      return true;
+    }
+    flat -= __shfl(ends, 63, kWave);
+  }
+  return false;
+}
+
+// The row and query block of grid block u: one block a row where no row has more.
+template <int ROWS>
+__device__ inline bool grid_block(const Attn4Args& a, int64_t u, int& row, int& qb) {
+  if (a.flat) return flat_block<ROWS>(a, u, row, qb);
+  row = static_cast<int>(u);
+  qb = 0;
+  return true;
+}
+
 // Waves a SIMD that the registers of an instantiation are for.
-constexpr int waves_per_simd(int np, int d, int mt) { return np == 3 ? (d == 256 ? 1 : 2) : d == 256 || mt == 2 ? 2 : KVHOT_W4; }
+constexpr int waves_per_simd(int np, int d, int mt) { return np == 3 ? (d == 256 ? 1 : 2) : d == 256 || mt == 2 ? 2 : 3; }
 
 template <class IO, class M, int NP, int D, int MT>
 __global__ void __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NP, D, MT))))
@@ -813,16 +856,15 @@ attn_4bit_kernel(Attn4Args a) {
   u /= a.hkv;
   const int part = static_cast<int>(u % a.parts);
   u /= a.parts;
-  const int qb = static_cast<int>(u % a.q_blocks);
-  const int row = static_cast<int>(u / a.q_blocks);
+  int row, qb;
   Block4 b;
-  if (!block_of<ROWS>(a, row, head, qb, b)) return;
+  if (!grid_block<ROWS>(a, u, row, qb) || !block_of<ROWS>(a, row, head, qb, b)) return;
   const int steps = (b.limit + kStep - 1) / kStep;
   const int step0 = part * a.part_steps, step1 = imin(steps, step0 + a.part_steps);
   if (part > 0 && step0 >= steps) return;
   u32x4 q[MT][NP][NJ];
   int lim[MT];
-  load_queries<IO, M, NP, D, MT, false>(a, b, 0, lane, q, lim);
+  load_queries<IO, M, NP, D, MT>(a, b, lane, q, lim);
   State4<D, MT> st;
   clear(st);
   // A step's keys are loaded while the step before is weighed, its values while
@@ -864,373 +906,13 @@ attn_4bit_kernel(Attn4Args a) {
   if (wave != 0) return;
   join<D, MT>(st, lds, lane);
 
-  const int64_t w = ((static_cast<int64_t>(row) * a.q_blocks + qb) * a.parts + part) * a.hkv + head;
-  finish<IO, D, MT>(a, b, 0, steps <= a.part_steps, w * ROWS, lane, st,
-                    [&](int c, int r) { return 2 * pair_of<D>(4 * (lane >> 4) + r, c >> 1) + (c & 1); });
-}
-
-// ------------------------------------------------------------------ prompts --
-
-// Rows of more than kDirect (query, head) pairs a kv head: a work-group has a block
-// of ROWS m-rows, 16 * MT a wave, and its waves convert each step's 64 keys into LDS
-// together, once for all of them, where the kernel above would convert them once a
-// wave.  K goes in row by row, V transposed (its codes lie that way): both are
-// then 16-byte reads of an operand.  Two buffers: a step is converted while the
-// one before is attended, one barrier a step.
-//
-// Rows of LDS are an odd number of 16-byte pieces, so that 16 of them at one
-// column lie in 16 different bank groups.  Token 32 a + 8 x + 4 y + z (z < 4) of a
-// step is K's LDS row 32 a + 16 y + 4 x + z: rows 4 g .. 4 g + 3 of the score tiles
-// 2 a and 2 a + 1 are then the eight tokens from 32 a + 8 g on, the k index of V's
-// product in order.  V's rows are the even elements, then the odd ones.
-constexpr int kDirect = KVHOT_DIRECT;
-
-template <int D>
-struct Prompt4 {
-  static constexpr int MT = D == 256 ? 1 : 2;     // m-row tiles of a wave
-  static constexpr int W = KVHOT_PW;              // waves
-  static constexpr int ROWS = 16 * MT * W;        // m-rows of a work-group
-  static constexpr int KP = 2 * D + 16;           // bytes of an LDS row of K
-  static constexpr int VP = 2 * kStep + 16;       // and of V^T
-  static constexpr int BUFFER = kStep * KP + D * VP;
-  static constexpr int UNITS = 2 * kStep * (D / 32);          // 16-byte loads of a step: K, then V
-  static constexpr int PER = (UNITS + 64 * W - 1) / (64 * W); // of a thread
-};
-
-// What a thread converts of a step: units threadIdx.x + i * 64 * W, those of K (token,
-// group) before those of V (record, pair).
-template <int D>
-struct Raw4 {
-  u32x4 code[Prompt4<D>::PER], scale[Prompt4<D>::PER];
-};
-template <int D>
-struct Ids4 {
-  int32_t id[Prompt4<D>::PER];
-};
-
-template <int D>
-__device__ inline bool unit(int i, bool& is_v, int& x) {
-  using P = Prompt4<D>;
-  const int u = static_cast<int>(threadIdx.x) + i * 64 * P::W;
-  is_v = u >= P::UNITS / 2;
-  x = is_v ? u - P::UNITS / 2 : u;
-  return P::UNITS % (64 * P::W) == 0 || u < P::UNITS;
-}
-
-template <int D>
-__device__ inline int slice_of(bool is_v, int x, int step, int last) {
-  return imin(step * 4 + (is_v ? x / (D / 2) : x / (D / 32) / 16), last);
-}
-
-// The block ids of a step, which its loads wait for: asked for a step before them.
-template <int D>
-__device__ inline void load_ids(const Attn4Args& a, const Block4& b, int step, Ids4<D>& ids) {
-  const int last = (b.limit + 15) / 16 - 1;
-  const int32_t* bt = a.bt + static_cast<int64_t>(b.row) * a.bt_stride;
-#pragma unroll
-  for (int i = 0; i < Prompt4<D>::PER; ++i) {
-    bool is_v;
-    int x;
-    if (!unit<D>(i, is_v, x)) continue;
-    const int slice = slice_of<D>(is_v, x, step, last);
-    ids.id[i] = bt[a.spb == 1 ? slice : slice / a.spb];
-  }
-}
-
-template <int D>
-__device__ inline void load_raw(const Attn4Args& a, const Block4& b, int step, const Ids4<D>& ids, Raw4<D>& raw) {
-  constexpr int NG = D / 32;
-  const int last = (b.limit + 15) / 16 - 1;
-#pragma unroll
-  for (int i = 0; i < Prompt4<D>::PER; ++i) {
-    bool is_v;
-    int x;
-    if (!unit<D>(i, is_v, x)) continue;
-    const char* rec = record_at<D>(a, b, ids.id[i], a.spb == 1 ? 0 : slice_of<D>(is_v, x, step, last) % a.spb);
-    if (is_v) {
-      const int pair = x % (D / 2);
-      raw.code[i] = *reinterpret_cast<const u32x4*>(rec + 8 * D + pair * 16);
-      raw.scale[i] = *reinterpret_cast<const u32x4*>(rec + 16 * D + D / 2 + (pair >> 4) * 16);
-    } else {
-      const int tok = x / NG % 16, g = x % NG;
-      raw.code[i] = *reinterpret_cast<const u32x4*>(rec + tok * (D / 2) + g * 16);
-      raw.scale[i].x = static_cast<uint8_t>(rec[16 * D + g * 16 + (tok & 3) * 4 + (tok >> 2)]);
-    }
-  }
-}
-
-// For a step that some m-row of the work-group does not see whole: NaN of V becomes
-// finite and is noted in `nan`, a bit for each of the 64 keys of a group; so does,
-// unnoted, whatever lies behind the last key that any of them sees.
-template <int D>
-__device__ inline void note_nan(Raw4<D>& raw, int base, int limit, uint32_t* nan) {
-#pragma unroll
-  for (int i = 0; i < Prompt4<D>::PER; ++i) {
-    bool is_v;
-    int x;
-    if (!unit<D>(i, is_v, x) || !is_v) continue;
-    const int slice = x / (D / 2), pair = x % (D / 2), left = limit - base - 16 * slice;
-    uint32_t bits = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      uint32_t sc = raw.scale[i][w];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint32_t sh = 8 * t;
-        const bool seen = 4 * w + t < left, bad = ((sc >> sh) & 255) == 255;
-        if (seen && bad) bits |= 1u << (4 * w + t);
-        if (!seen || bad) sc = (sc & ~(255u << sh)) | 127u << sh;
-      }
-      raw.scale[i][w] = sc;
-    }
-    if (bits && (pair & 15) == 0) atomicOr(nan + (pair >> 4) * 2 + (slice >> 1), bits << (16 * (slice & 1)));
-  }
-}
-
-// Converts a thread's share of a step into LDS.
-template <class M, int D>
-__device__ inline void convert(const Raw4<D>& raw, char* lds) {
-  using P = Prompt4<D>;
-  constexpr int NG = D / 32;
-#pragma unroll
-  for (int i = 0; i < P::PER; ++i) {
-    bool is_v;
-    int x;
-    if (!unit<D>(i, is_v, x)) continue;
-    if (!is_v) {
-      const int tok = x / NG, g = x % NG;
-      const int row = (tok & 32) | (tok & 4) << 2 | (tok & 24) >> 1 | (tok & 3);
-      const float s = scale_of(raw.scale[i].x);
-      char* p = lds + row * P::KP + g * 64;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(p + 16 * j) = codes8<M>(raw.code[i][j], s);
-    } else {
-      const int slice = x / (D / 2), pair = x % (D / 2);
-      char* p = lds + kStep * P::KP + pair * P::VP + slice * 32;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 lo, hi;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t code = raw.code[i][2 * h + w], sw = raw.scale[i][2 * h + w];
-          const uint32_t a0 = pair16<M, 0>(code, scale_in(sw, 0)), a1 = pair16<M, 1>(code, scale_in(sw, 1)),
-                         a2 = pair16<M, 2>(code, scale_in(sw, 2)), a3 = pair16<M, 3>(code, scale_in(sw, 3));
-          lo[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x05040100);
-          lo[2 * w + 1] = __builtin_amdgcn_perm(a3, a2, 0x05040100);
-          hi[2 * w] = __builtin_amdgcn_perm(a1, a0, 0x07060302);
-          hi[2 * w + 1] = __builtin_amdgcn_perm(a3, a2, 0x07060302);
-        }
-        *reinterpret_cast<u32x4*>(p + 16 * h) = lo;
-        *reinterpret_cast<u32x4*>(p + D / 2 * P::VP + 16 * h) = hi;
-      }
-    }
-  }
-}
-
-// Attends a step from LDS.
-template <class M, int D, bool MASKED>
-__device__ inline void attend_lds(const char* lds, const u32x4 (&q)[Prompt4<D>::MT][1][D / 32],
-                                  const int (&sees)[Prompt4<D>::MT], int base, float scale, int lane, const uint32_t* nan,
-                                  State4<D, Prompt4<D>::MT>& st) {
-  using P = Prompt4<D>;
-  constexpr int MT = P::MT, NJ = D / 32;
-  const int i = lane & 15, g = lane >> 4;
-  // Operands of the next tile are read while the matrix cores have this one's.
-  f32x4 sc[MT][4];
-  {
-    u32x4 k[2][NJ];
-    const char* at = lds + i * P::KP + g * 16;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) k[0][j] = *reinterpret_cast<const u32x4*>(at + j * 64);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (t < 3) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) k[(t + 1) & 1][j] = *reinterpret_cast<const u32x4*>(at + 16 * (t + 1) * P::KP + j * 64);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) sc[m][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) sc[m][t] = M::mfma(k[t & 1][j], q[m][0][j], sc[m][t]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  u32x4 p[MT][1][2];
-  const auto key = [](int t, int r) { return 32 * (t >> 1) + 4 * (t & 1) + r; };
-  probabilities<M, 1, D, MT, MASKED>(sc, sees, base + 8 * g, key, scale, st, p);
-  __builtin_amdgcn_sched_barrier(0);
-  {
-    u32x4 v[2][2];
-    const char* at = lds + kStep * P::KP + i * P::VP + g * 16;
-    v[0][0] = *reinterpret_cast<const u32x4*>(at);
-    v[0][1] = *reinterpret_cast<const u32x4*>(at + 64);
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      if (c + 1 < D / 16) {
-        v[(c + 1) & 1][0] = *reinterpret_cast<const u32x4*>(at + 16 * (c + 1) * P::VP);
-        v[(c + 1) & 1][1] = *reinterpret_cast<const u32x4*>(at + 16 * (c + 1) * P::VP + 64);
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) st.o[m][c] = M::mfma(v[c & 1][u], p[m][0][u], st.o[m][c]);
-      if (c & 1) __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  if (MASKED) {
-#pragma unroll
-    for (int x = 0; x < NJ; ++x)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t bits = __builtin_amdgcn_readfirstlane(nan[2 * x + h]);
-        while (bits) {
-          const int at = base + 32 * h + __builtin_ctz(bits);
-          bits &= bits - 1;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            if (at < sees[m]) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) st.o[m][x][r] = st.o[m][NJ + x][r] = __builtin_nanf("");
-            }
-        }
-      }
-  }
-}
-
-// The query block `flat` of the rows that take this kernel: of each 64 rows the one
-// with the most keys first, and its last block first (causal blocks' work grows
-// along a row), so that the longest start first.
-template <int ROWS>
-__device__ inline bool flat_block(const Attn4Args& a, int head, int64_t flat, int& row, int& qb) {
-  const int lane = threadIdx.x & 63;
-  for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
-    int64_t mine = 0;
-    int keys = -1;
-    if (r0 + lane < a.num_rows) {
-      const int64_t n = static_cast<int64_t>(imin(a.q_lens[r0 + lane], a.max_q)) * a.group;
-      if (n > kDirect) {
-        mine = (n + ROWS - 1) / ROWS;
-        keys = a.k_lens[r0 + lane];
-      }
-    }
-    int rank = 0;  // rows that come before the lane's
-    for (uint64_t left = __ballot(mine > 0); left; left &= left - 1) {
-      const int other = __builtin_ctzll(left), k = __builtin_amdgcn_readlane(keys, other);
-      rank += k > keys || (k == keys && other < lane) ? 1 : 0;
-    }
-    // (lanes without blocks go behind the others, in their order)
-    const uint64_t with = __ballot(mine > 0);
-    if (mine == 0) rank = __popcll(with) + __popcll(~with & ((uint64_t{1} << lane) - 1));
-    const int from = __builtin_amdgcn_ds_permute(rank * 4, lane);  // the row of rank `lane`
-    mine = __shfl(mine, from, kWave);
-    int64_t ends = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t x = __shfl_up(ends, o, kWave);
-      if (lane >= o) ends += x;
-    }
-    const uint64_t after = __ballot(ends > flat);
-    if (after) {
-      const int at = __builtin_ctzll(after);
-      row = r0 + __shfl(from, at, kWave);
-      qb = static_cast<int>(__shfl(ends, at, kWave) - 1 - flat);
-      row = __builtin_amdgcn_readfirstlane(row);
-      qb = __builtin_amdgcn_readfirstlane(qb);
-      return true;
-    }
-    flat -= __shfl(ends, 63, kWave);
-  }
-  return false;
-}
-
-// A barrier for what goes through LDS: loads from memory stay on their way.
-__device__ inline void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
-template <class IO, class M, int D>
-__global__ void __launch_bounds__(64 * Prompt4<D>::W) __attribute__((amdgpu_waves_per_eu(2)))
-prompt_4bit_kernel(Attn4Args a) {
-  using P = Prompt4<D>;
-  constexpr int MT = P::MT, NJ = D / 32, NG = D / 32;
-  __shared__ char lds[2][P::BUFFER];
-  __shared__ uint32_t nan[3][NG * 2];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int64_t u = blockIdx.x;
-  const int head = static_cast<int>(u % a.hkv);
-  u /= a.hkv;
-  const int part = static_cast<int>(u / a.blocks);
-  u %= a.blocks;
-  int row, qb;
-  if (!flat_block<P::ROWS>(a, head, u, row, qb)) return;
-  Block4 b;
-  if (!block_of<P::ROWS>(a, row, head, qb, b)) return;
-  const int steps = (b.limit + kStep - 1) / kStep;
-  const int step0 = part * a.part_steps, step1 = imin(steps, step0 + a.part_steps);
-  if (part > 0 && step0 >= steps) return;
-  const int first = 16 * MT * wave;  // the wave's m-rows in the block
-
-  u32x4 q[MT][1][NJ];
-  int lim[MT], least = b.limit, most = 0;
-  load_queries<IO, M, 1, D, MT, true>(a, b, first, lane, q, lim);
-  if (first < b.rows) {
-    least = sees(a, b, b.first + first);
-    most = sees(a, b, b.first + imin(first + 16 * MT, b.rows) - 1);
-  }
-  State4<D, MT> st;
-  clear(st);
-  if (threadIdx.x < 3 * NG * 2) (&nan[0][0])[threadIdx.x] = 0;
-  Raw4<D> raw;
-  Ids4<D> ids;
-  const int full = b.least / kStep;  // steps that every m-row of the work-group sees whole
-  if (step0 < step1) {
-    load_ids<D>(a, b, step0, ids);
-    load_raw<D>(a, b, step0, ids, raw);
-    load_ids<D>(a, b, imin(step0 + 1, step1 - 1), ids);
-  }
-  __syncthreads();
-  if (step0 < step1) {
-    if (step0 >= full) note_nan<D>(raw, step0 * kStep, b.limit, nan[0]);
-    convert<M, D>(raw, lds[0]);
-    load_raw<D>(a, b, imin(step0 + 1, step1 - 1), ids, raw);
-    load_ids<D>(a, b, imin(step0 + 2, step1 - 1), ids);
-  }
-  __syncthreads();
-  int buf = 0, slot = 0;
-  for (int s = step0; s < step1; ++s) {
-    // (Every thread of the work-group passes here the same number of times.)
-    const int next = slot == 2 ? 0 : slot + 1, after = next == 2 ? 0 : next + 1;
-    if (threadIdx.x < NG * 2) nan[after][threadIdx.x] = 0;
-    if (s + 1 < step1) {
-      if (s + 1 >= full) note_nan<D>(raw, (s + 1) * kStep, b.limit, nan[next]);
-      convert<M, D>(raw, lds[buf ^ 1]);
-      load_raw<D>(a, b, imin(s + 2, step1 - 1), ids, raw);
-      load_ids<D>(a, b, imin(s + 3, step1 - 1), ids);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (s * kStep < most) {  // some m-row of the wave sees some of it
-      if (s * kStep + kStep <= least && s < full)
-        attend_lds<M, D, false>(lds[buf], q, lim, s * kStep, a.scale, lane, nan[slot], st);
-      else
-        attend_lds<M, D, true>(lds[buf], q, lim, s * kStep, a.scale, lane, nan[slot], st);
-    }
-    lds_barrier();
-    buf ^= 1;
-    slot = next;
-  }
-  if (first >= b.rows) return;
   const int64_t w = (u * a.parts + part) * a.hkv + head;
-  finish<IO, D, MT>(a, b, first, steps <= a.part_steps, w * P::ROWS, lane, st,
-                    [&](int c, int r) { return 2 * (16 * (c % NJ) + 4 * (lane >> 4) + r) + c / NJ; });
+  finish<IO, D, MT>(a, b, steps <= a.part_steps, w * ROWS, lane, st);
 }
 
 // Joins the parts of the query blocks that were cut: one wave an m-row, eight
 // parts on their way at a time.
-template <class IO, int D, int ROWS, bool PROMPT>
+template <class IO, int D, int ROWS>
 __global__ void __launch_bounds__(256)
 merge_4bit_kernel(Attn4Args a) {
   constexpr int PER = (D + 63) / 64, AHEAD = 8;
@@ -1240,18 +922,16 @@ merge_4bit_kernel(Attn4Args a) {
   u /= ROWS / 4;
   const int head = static_cast<int>(u % a.hkv);
   u /= a.hkv;
-  const int64_t block = u;  // of the workspace
-  int row = static_cast<int>(u / a.q_blocks), qb = static_cast<int>(u % a.q_blocks);
-  if (PROMPT && !flat_block<ROWS>(a, head, u, row, qb)) return;
+  int row, qb;
   Block4 b;
   const int m = quarter * 4 + wave;
-  if (!block_of<ROWS>(a, row, head, qb, b) || m >= b.rows || (!PROMPT && b.all > a.direct)) return;
+  if (!grid_block<ROWS>(a, u, row, qb) || !block_of<ROWS>(a, row, head, qb, b) || m >= b.rows) return;
   const int steps = (b.limit + kStep - 1) / kStep;
   const int parts = (steps + a.part_steps - 1) / a.part_steps;
   const int mr = b.first + m;
   const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
   if (parts <= 1 || tok < 0 || tok >= a.total_query) return;
-  const int64_t w0 = block * a.parts * a.hkv + head;
+  const int64_t w0 = u * a.parts * a.hkv + head;
   float ref = -INFINITY, sum = 0, x[PER] = {};
   for (int p0 = 0; p0 < parts; p0 += AHEAD) {
     float l[AHEAD], y[AHEAD][PER];
@@ -1345,56 +1025,40 @@ spread_nan_4bit_kernel(Nan4Args n, int d) {
 
 constexpr int64_t kWholeSteps = 128;
 
-// Split of a call's rows that take one of the two kernels: query blocks (of a row
-// in the first, of all rows in the second; 0: no such rows), parts, key steps of
-// a part, and the workspace: partials, then their logarithms.
+// Split of a call: tiles of 16 m-rows of a query block, blocks (of all rows), parts,
+// key steps of a part, and the workspace: partials, then their logarithms.
 struct Split4 {
-  int32_t q_blocks = 0, parts = 1, part_steps = 1;
-  int64_t blocks = 0, rows = 0, ws_bytes = 0;
-  void cut(int64_t d, int64_t steps, int64_t n, int64_t per) {
-    part_steps = static_cast<int32_t>(std::max<int64_t>(per, 1));
-    parts = static_cast<int32_t>(std::max<int64_t>((steps + part_steps - 1) / part_steps, 1));
-    ws_bytes = parts > 1 ? n * parts * rows * (d + 1) * 4 : 0;
-    ws_bytes = (ws_bytes + 255) / 256 * 256;
-  }
-};
-struct Plan4 {
-  Split4 direct, prompt;
-  int64_t limit;  // m-rows of a row up to which it takes the first kernel
+  int32_t mt, flat, parts, part_steps;
+  int64_t blocks, ws_bytes;
 };
 
-static Plan4 plan_4bit(int64_t rows, int64_t total, int64_t max_q, int64_t max_k, int64_t group, int64_t hkv, int64_t d,
-                       int dtype) {
-  Plan4 p;
+static Split4 split_4bit(int64_t rows, int64_t total, int64_t max_q, int64_t max_k, int64_t group, int64_t hkv, int64_t d,
+                         int dtype) {
+  Split4 s;
   const int64_t longest = max_q * group, steps = (max_k + kStep - 1) / kStep;
-  // (fp32 has the first kernel only: its queries and probabilities are three
-  // values each, for which the second has no registers.)
-  p.limit = dtype == KVHOT_F32 ? INT64_MAX : kDirect;
-  const int64_t m = std::min(longest, p.limit);
-  Split4& a = p.direct;
-  a.rows = 16;
-  a.q_blocks = static_cast<int32_t>((m + a.rows - 1) / a.rows);
-  a.blocks = rows * a.q_blocks;
+  // no more blocks than the call's queries fill, and one more for each row
+  const auto blocks = [&](int64_t m) {
+    return longest <= m ? rows : std::min(rows * ((longest + m - 1) / m), total * group / m + std::min(rows, total));
+  };
+  // Two tiles share a step's conversion, in registers for two waves a SIMD, not
+  // three: from 1024 blocks of one on (bf16, head_dim 128, 32 / 8 heads, us with
+  // one and two: 8 rows of 32 queries on 2048 keys 22 / 39, of 64 37 / 31, of 512
+  // 225 / 186; 300 queries on 5000 keys 54 / 61; 2048 on 2048 82 / 73).
+  s.mt = longest > 16 && dtype != KVHOT_F32 && d <= 128 && blocks(16) * hkv >= 1024 ? 2 : 1;
+  s.flat = longest > 16 * s.mt;
+  s.blocks = blocks(16 * s.mt);
   // Blocks that give each of 256 CUs two work-groups are left whole up to
   // kWholeSteps steps (64 rows of 128-2048 keys: 23.6 us, in two parts 25.7 and
   // a merge of 4.8); fewer are cut for four work-groups a CU, of which three
   // fit: rows are ragged, and the parts behind a short row's end are empty
   // (24 rows of up to 6000 keys: 20.9 us, 24.9 when cut for three).
-  int64_t n = a.blocks * hkv;
-  int64_t parts = n >= 512 ? 1 : (1024 + n - 1) / n;
-  a.cut(d, steps, n, std::min<int64_t>(std::max<int64_t>((steps + parts - 1) / parts, 2 * kWaves4), kWholeSteps));
-  if (longest > p.limit) {
-    Split4& b = p.prompt;
-    b.rows = d == 256 ? Prompt4<256>::ROWS : Prompt4<128>::ROWS;
-    // no more blocks than the call's queries fill, and one more for each row
-    // that takes this kernel
-    const int64_t pairs = total * group;
-    b.blocks = std::min(rows * ((longest + b.rows - 1) / b.rows), pairs / b.rows + std::min(rows, pairs / (p.limit + 1)));
-    n = std::max<int64_t>(b.blocks * hkv, 1);
-    parts = std::max<int64_t>(1, 512 / n);
-    b.cut(d, steps, n, std::max<int64_t>((steps + parts - 1) / parts, 4));
-  }
-  return p;
+  const int64_t n = std::max<int64_t>(s.blocks * hkv, 1);
+  const int64_t parts = n >= 512 ? 1 : (1024 + n - 1) / n;
+  const int64_t per = std::min<int64_t>(std::max<int64_t>((steps + parts - 1) / parts, 2 * kWaves4), kWholeSteps);
+  s.part_steps = static_cast<int32_t>(per);
+  s.parts = static_cast<int32_t>(std::max<int64_t>((steps + per - 1) / per, 1));
+  s.ws_bytes = s.parts > 1 ? n * s.parts * 16 * s.mt * (d + 1) * 4 : 0;
+  return s;
 }
 
 }  // namespace kvhot
@@ -1528,59 +1192,47 @@ static int check_attention(int64_t rows, int64_t total, int64_t max_q, int64_t m
   return 0;
 }
 
-extern "C" int64_t kvhot_paged_attention_4bit_workspace_bytes(int64_t num_rows, int64_t total_query, int64_t max_q_len,
+extern "C" int64_t kvhot_paged_attention_4bit_workspace_bytes(int64_t num_rows, int64_t sum_q_lens, int64_t max_q_len,
                                                               int64_t max_k_len, int64_t num_q_heads,
                                                               int64_t num_kv_heads, int64_t head_dim, int dtype) {
   clear_error();
-  if (int e = check_attention(num_rows, total_query, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
+  if (int e = check_attention(num_rows, sum_q_lens, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
     return e;
-  if (num_rows == 0 || total_query == 0 || max_q_len == 0) return 0;
-  const Plan4 p = plan_4bit(num_rows, total_query, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
-                            dtype);
-  return p.direct.ws_bytes + p.prompt.ws_bytes;
+  if (num_rows == 0 || sum_q_lens == 0 || max_q_len == 0) return 0;
+  return split_4bit(num_rows, sum_q_lens, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads, head_dim, dtype)
+      .ws_bytes;
 }
 
 namespace {
 
-// One of the two kernels, then the merge of what it cut into parts; the split's
-// workspace begins at ws.
-int launch_split(const Split4& sp, Attn4Args& a, char* ws, int64_t d, hipStream_t s, void (*kernel)(Attn4Args), int waves,
-                 void (*merge)(Attn4Args)) {
+template <class IO, class M, int NP, int D, int MT>
+int launch_4bit(const Split4& sp, const Attn4Args& a, hipStream_t s) {
   const int64_t blocks = sp.blocks * a.hkv;
-  if (blocks == 0) return 0;
-  if (blocks * std::max<int64_t>(sp.parts, sp.rows / 4) > 0x7fffffff)
+  if (blocks * std::max<int64_t>(sp.parts, 4 * MT) > 0x7fffffff)
     return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
-  a.q_blocks = std::max(sp.q_blocks, 1);
-  a.parts = sp.parts;
-  a.part_steps = sp.part_steps;
-  a.blocks = sp.blocks;
-  a.ws_o = reinterpret_cast<float*>(ws);
-  a.ws_lse = a.ws_o ? a.ws_o + blocks * sp.parts * sp.rows * d : nullptr;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(blocks * sp.parts)), dim3(64 * waves), 0, s, a);
+  hipLaunchKernelGGL((attn_4bit_kernel<IO, M, NP, D, MT>), dim3(static_cast<uint32_t>(blocks * sp.parts)),
+                     dim3(64 * kWaves4), 0, s, a);
   if (int e = launch_status("paged_attention_4bit")) return e;
   if (sp.parts == 1) return 0;
-  hipLaunchKernelGGL(merge, dim3(static_cast<uint32_t>(blocks * (sp.rows / 4))), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks * (4 * MT))), dim3(256), 0, s,
+                     a);
   return launch_status("paged_attention_4bit merge");
 }
 
 template <class IO, class M, int NP, int D>
-int launch_4bit(const Plan4& p, Attn4Args& a, char* ws, hipStream_t s) {
-  int e = launch_split(p.direct, a, ws, D, s, attn_4bit_kernel<IO, M, NP, D, 1>, kWaves4, merge_4bit_kernel<IO, D, 16, false>);
-  if constexpr (NP == 1) {
-    if (e == 0 && p.prompt.blocks > 0)
-      e = launch_split(p.prompt, a, ws ? ws + p.direct.ws_bytes : nullptr, D, s, prompt_4bit_kernel<IO, M, D>, Prompt4<D>::W,
-                       merge_4bit_kernel<IO, D, Prompt4<D>::ROWS, true>);
-  }
-  return e;
+int launch_4bit(const Split4& sp, const Attn4Args& a, hipStream_t s) {
+  if constexpr (NP == 1 && D <= 128)
+    if (sp.mt == 2) return launch_4bit<IO, M, NP, D, 2>(sp, a, s);
+  return launch_4bit<IO, M, NP, D, 1>(sp, a, s);
 }
 
 template <class IO, class M, int NP>
-int launch_4bit(const Plan4& p, Attn4Args& a, int64_t d, char* ws, hipStream_t s) {
+int launch_4bit(const Split4& sp, const Attn4Args& a, int64_t d, hipStream_t s) {
   switch (d) {
-    case 64: return launch_4bit<IO, M, NP, 64>(p, a, ws, s);
-    case 96: return launch_4bit<IO, M, NP, 96>(p, a, ws, s);
-    case 128: return launch_4bit<IO, M, NP, 128>(p, a, ws, s);
-    default: return launch_4bit<IO, M, NP, 256>(p, a, ws, s);
+    case 64: return launch_4bit<IO, M, NP, 64>(sp, a, s);
+    case 96: return launch_4bit<IO, M, NP, 96>(sp, a, s);
+    case 128: return launch_4bit<IO, M, NP, 128>(sp, a, s);
+    default: return launch_4bit<IO, M, NP, 256>(sp, a, s);
   }
 }
 
@@ -1667,8 +1319,8 @@ extern "C" int kvhot_paged_attention_4bit(
     const void* q, const int64_t q_strides[3], const void* cache, int64_t block_stride_bytes, void* out,
     const int64_t out_strides[3], float* lse, const int64_t lse_strides[2], const int32_t* block_table,
     int64_t bt_row_stride, const int32_t* q_lens, const int32_t* k_lens, const int32_t* q_starts,
-    const int32_t* q_pos_offsets, int64_t num_rows, int64_t total_query, int64_t max_q_len, int64_t max_k_len,
-    int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks, float scale,
+    const int32_t* q_pos_offsets, int64_t num_rows, int64_t total_query, int64_t sum_q_lens, int64_t max_q_len,
+    int64_t max_k_len, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks, float scale,
     int attn_flags, int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   if (int e = check_attention(num_rows, total_query, max_q_len, max_k_len, num_q_heads, num_kv_heads, head_dim, dtype))
@@ -1676,7 +1328,8 @@ extern "C" int kvhot_paged_attention_4bit(
   if (int e = check_pool("paged_attention_4bit", cache, block_stride_bytes, num_kv_heads, head_dim, block_size, num_blocks))
     return e;
   if (attn_flags & ~KVHOT_CAUSAL) return set_error(KVHOT_EINVAL, "paged_attention_4bit: unknown attn_flags");
-  if (num_rows == 0 || total_query == 0 || max_q_len == 0) return 0;
+  if (sum_q_lens < 0 || sum_q_lens > total_query) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sum_q_lens");
+  if (num_rows == 0 || sum_q_lens == 0 || max_q_len == 0) return 0;
   if (!q || !out || !q_strides || !out_strides || !q_lens || !k_lens || !q_starts || !q_pos_offsets ||
       (lse && !lse_strides) || (!block_table && bt_row_stride > 0 && max_k_len > 0))
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: null pointer");
@@ -1684,19 +1337,22 @@ extern "C" int kvhot_paged_attention_4bit(
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: head_dim must be the innermost, unit-stride dim");
   if (bt_row_stride < 0 || num_rows > 0x7fffffff) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
   if (num_blocks == 0 && max_k_len > 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: keys but no blocks");
-  const Plan4 plan = plan_4bit(num_rows, total_query, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads,
+  const Split4 sp = split_4bit(num_rows, sum_q_lens, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads,
                                head_dim, dtype);
-  const int64_t need = plan.direct.ws_bytes + plan.prompt.ws_bytes;
-  if (need > 0 && (!workspace || workspace_bytes < need))
+  if (sp.ws_bytes > 0 && (!workspace || workspace_bytes < sp.ws_bytes))
     return set_error(KVHOT_EWORKSPACE, "paged_attention_4bit: workspace missing or too small");
   Attn4Args a = args_4bit(q, q_strides, cache, block_stride_bytes, out, out_strides, lse, lse_strides, block_table,
                           bt_row_stride, q_lens, k_lens, q_starts, q_pos_offsets, num_rows, total_query, max_q_len, max_k_len,
                           num_q_heads, num_kv_heads, block_size, num_blocks, scale, attn_flags, dtype);
-  a.direct = plan.limit;
+  a.flat = sp.flat;
+  a.parts = sp.parts;
+  a.part_steps = sp.part_steps;
+  a.ws_o = static_cast<float*>(workspace);
+  a.ws_lse = a.ws_o ? a.ws_o + sp.blocks * num_kv_heads * sp.parts * 16 * sp.mt * head_dim : nullptr;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case KVHOT_F32: return launch_4bit<F32, BF16, 3>(plan, a, head_dim, static_cast<char*>(workspace), s);
-    case KVHOT_F16: return launch_4bit<F16, F16, 1>(plan, a, head_dim, static_cast<char*>(workspace), s);
-    default: return launch_4bit<BF16, BF16, 1>(plan, a, head_dim, static_cast<char*>(workspace), s);
+    case KVHOT_F32: return launch_4bit<F32, BF16, 3>(sp, a, head_dim, s);
+    case KVHOT_F16: return launch_4bit<F16, F16, 1>(sp, a, head_dim, s);
+    default: return launch_4bit<BF16, BF16, 1>(sp, a, head_dim, s);
   }
 }

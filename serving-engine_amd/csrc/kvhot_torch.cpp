@@ -425,7 +425,7 @@ PyObject* py_read4(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // attention4(q, blocks, metadata, hq, hkv, scale, causal, workspaces, prompt_pairs) -> (o, l) | None
 //   (None where the host knows of a row that may have that many (query, head) pairs
-//   a kv head: prompts are planned in Python.)
+//   a kv head, unless the step's plan is there and has no prompts.)
 PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return or_none([&]() -> PyObject* {
     Tensor q, kv, q_lens, k_lens, q_starts, q_offs, bt, ws;
@@ -451,7 +451,18 @@ PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !as_int(PyDict_GetItemWithError(meta, g_names.max_k_len), max_k))
       return nullptr;
     PyObject* host = PyDict_GetItemWithError(meta, g_names.host_q_lens);
-    if (host && host != Py_None && max_q * (hq / hkv) >= prompt) return nullptr;
+    if (host && host != Py_None && dt != KVHOT_F32 && max_q * (hq / hkv) >= prompt) {
+      PyObject* plans = PyDict_GetItemWithError(meta, g_names.schedules);
+      if (!plans || !PyDict_CheckExact(plans)) return nullptr;
+      char name[16];
+      snprintf(name, sizeof name, "cuda:%d", static_cast<int>(d.index()));
+      PyObject* key = Py_BuildValue("(sLLLLis)", "prompts4", (long long)hq, (long long)hkv, (long long)q.size(2),
+                                    (long long)(kv.size(1) * 16), dt, name);
+      if (!key) return nullptr;
+      PyObject* hit = PyDict_GetItemWithError(plans, key);
+      Py_DECREF(key);
+      if (hit != Py_None) return nullptr;
+    }
     const int64_t need = g_workspace_bytes4(rows, q.size(0), max_q, max_k, hq, hkv, q.size(2), dt);
     void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
     if (need < 0 || (need > 0 && !stream_workspace(a[7], d, stream, need, ws))) return nullptr;
@@ -463,7 +474,7 @@ PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto i32 = [](const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); };
     const int status = without_gil([&] {
       return g_attention4(q.data_ptr(), qs, kv.data_ptr(), kv.stride(0), o.data_ptr(), os, static_cast<float*>(l.data_ptr()),
-                          ls, i32(bt), bt_stride, i32(q_lens), i32(k_lens), i32(q_starts), i32(q_offs), rows, q.size(0),
+                          ls, i32(bt), bt_stride, i32(q_lens), i32(k_lens), i32(q_starts), i32(q_offs), rows, q.size(0), q.size(0),
                           max_q, max_k, hq, hkv, q.size(2), kv.size(1) * 16, kv.size(0), scale, flags, dt,
                           ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? ws.numel() : 0, stream);
     });

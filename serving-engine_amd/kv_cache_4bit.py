@@ -225,24 +225,25 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     bt_stride = int(metadata.get("block_table_row_stride", bt.shape[1] if bt.dim() == 2 else 0))
     max_q = _host_max(metadata, "max_q_len", "q_lens")
     max_k = _host_max(metadata, "max_k_len", "k_lens")
-    plan = _prompts(metadata, device, num_q_heads // num_kv_heads, spb * RECORD_TOKENS)
+    plan = _prompts(metadata, device, num_q_heads, num_kv_heads, head_dim, spb * RECORD_TOKENS, q.dtype)
     with torch.cuda.device(device):
         if plan is None:
-            _attend(q, kv_blocks, metadata, q_lens, max_q, max_k, bt_stride, scale, is_causal, o, l)
+            _attend(q, kv_blocks, metadata, q_lens, total_query, max_q, max_k, bt_stride, scale, is_causal, o, l)
         else:
             if plan.max_q:
-                _attend(q, kv_blocks, metadata, plan.q_lens, plan.max_q, plan.max_k, bt_stride, scale, is_causal, o, l)
+                _attend(q, kv_blocks, metadata, plan.q_lens, plan.sum_q, plan.max_q, plan.max_k, bt_stride, scale, is_causal,
+                        o, l)
             _attend_prompts(q, kv_blocks, metadata, plan, bt_stride, scale, is_causal, o, l)
     return o, l
 
 
-def _attend(q, kv_blocks, metadata, q_lens, max_q, max_k, bt_stride, scale, is_causal, o, l):
+def _attend(q, kv_blocks, metadata, q_lens, sum_q, max_q, max_k, bt_stride, scale, is_causal, o, l):
     """kvhot_paged_attention_4bit of the rows that have queries in q_lens."""
     lib, device = _lib.load(), q.device
     total_query, hq, head_dim = q.shape
     num_blocks, spb, hkv, _ = kv_blocks.shape
     num_rows, dtype, stream = q_lens.shape[0], _lib.dtype_code(q.dtype), _lib.stream_handle(device)
-    need = lib.kvhot_paged_attention_4bit_workspace_bytes(num_rows, total_query, max_q, max_k, hq, hkv, head_dim, dtype)
+    need = lib.kvhot_paged_attention_4bit_workspace_bytes(num_rows, sum_q, max_q, max_k, hq, hkv, head_dim, dtype)
     if need < 0:
         _lib.check(int(need), "kvhot_paged_attention_4bit_workspace_bytes")
     ws = _workspace(device, stream, need)
@@ -251,34 +252,45 @@ def _attend(q, kv_blocks, metadata, q_lens, max_q, max_k, bt_stride, scale, is_c
         o.data_ptr(), _lib.i64_array(o.stride()), l.data_ptr(), _lib.i64_array(l.stride()),
         metadata["block_table"].data_ptr(), bt_stride, q_lens.data_ptr(), metadata["k_lens"].data_ptr(),
         metadata["q_starts"].data_ptr(), metadata["q_pos_offsets"].data_ptr(),
-        num_rows, total_query, max_q, max_k, hq, hkv, head_dim, spb * RECORD_TOKENS, num_blocks,
+        num_rows, total_query, sum_q, max_q, max_k, hq, hkv, head_dim, spb * RECORD_TOKENS, num_blocks,
         float(scale), _lib.KVHOT_CAUSAL if is_causal else 0, dtype,
         ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, stream)
     _lib.check(status, "kvhot_paged_attention_4bit")
 
 
 class _Prompts:
-    """What a step's calls know of its prompts (rows of at least PROMPT_PAIRS
-    (query, head) pairs a kv head), planned once: ``meta``, the metadata of those
+    """What a step's calls know of its prompts (rows that are attended over dense
+    copies of their keys), planned once: ``meta``, the metadata of those
     rows alone over a pool of their own keys' copies, block after block; ``slots``
     [16 * blocks], where those keys are (-1 behind a row's end); ``rows``, their
     rows in the step's block table; ``q_lens``, the step's with theirs 0, and the
     bounds of the rows that are left."""
 
 
-# (query, head) pairs a kv head from which a row is attended over dense copies.
+# A row with so many (query, head) pairs a kv head has its keys converted again for
+# every 32 of them; copied once instead, they serve the 16-bit pools' attention,
+# which then takes less time a pair.  The copies, the NaN's launch and the calls
+# from Python cost about 50 us more: worth it from PROMPT_FLOPS on, all such rows
+# together (bf16, 32 / 8 heads of 128, us a call from the 4-bit cache and over
+# copies: 8 rows of 128 queries on 2048 keys, 32 GFLOP, 57 / 77, of 256, 62 GFLOP,
+# 103 / 92, of 512 186 / 149; 300 queries on 5000 keys, 24 GFLOP, 54 / 58; 16 / 4
+# heads of 256: 82 / 82, 155 / 108, 81 / 66).  In fp32, where the 4-bit kernel
+# multiplies in three bf16 parts and the other on the fp32 matrix cores, never:
+# 8 rows of 256 queries at 8 / 2 heads of 64 38 / 127.
 PROMPT_PAIRS = 512
+PROMPT_FLOPS = 35e9
 # Bytes that a call's copies may take.
 PROMPT_BYTES = 8 << 30
 
 
-def _prompts(metadata, device, group, block_size):
+def _prompts(metadata, device, hq, hkv, d, block_size, dtype):
     """The step's _Prompts, planned from the host copies of its lengths and kept in
     the metadata; None without host copies or prompts."""
-    host_q = metadata.get("host_q_lens")
-    if host_q is None or _host_max(metadata, "max_q_len", "q_lens") * group < PROMPT_PAIRS:
+    host_q, group = metadata.get("host_q_lens"), hq // hkv
+    if (host_q is None or dtype == torch.float32
+            or _host_max(metadata, "max_q_len", "q_lens") * group < PROMPT_PAIRS):
         return None
-    key = ("prompts4", group, block_size, str(device))
+    key = ("prompts4", hq, hkv, d, block_size, _lib.dtype_code(dtype), str(device))
     cache = metadata.setdefault("_schedules", {})
     if key in cache:
         hit = cache[key]
@@ -288,12 +300,13 @@ def _prompts(metadata, device, group, block_size):
         return None  # (as _schedule: a copy from here would be replayed)
     host_k, host_off = metadata["host_k_lens"], metadata["host_q_pos_offsets"]
     rows = np.flatnonzero((host_q.astype(np.int64) * group >= PROMPT_PAIRS) & (host_k > 0))
-    if not rows.size:
+    q_lens, k_lens = host_q[rows].astype(np.float64), host_k[rows].astype(np.int64)
+    flops = 4.0 * hq * d * float((q_lens * (k_lens - q_lens / 2)).sum())  # causal
+    blocks = -(-k_lens // BLOCK_SIZE)
+    if flops < PROMPT_FLOPS or int(blocks.sum()) * BLOCK_SIZE * hkv * d * 4 > PROMPT_BYTES:
         cache[key] = None
         return None
-    r, n = len(host_q), len(rows)
-    k_lens = host_k[rows].astype(np.int64)
-    blocks = -(-k_lens // BLOCK_SIZE)
+    n = len(rows)
     ends = np.cumsum(blocks)
     total, width = int(ends[-1]), int(blocks.max())
     table = np.zeros((n, width), dtype=np.int32)
@@ -319,7 +332,7 @@ def _prompts(metadata, device, group, block_size):
     p = _Prompts()
     p.q_lens, p.rows, p.slots = dev[0], dev[5], buf[at[-1] + pad:].view(torch.int64)
     p.blocks = total
-    p.max_q = int(short.max()) if left.size else 0
+    p.sum_q, p.max_q = int(short[left].sum()), int(short.max()) if left.size else 0
     p.max_k = int(host_k[left].max()) if left.size else 0
     p.meta = dict(zip(("q_lens", "k_lens", "q_starts", "q_pos_offsets"), dev[1:5]))
     p.meta.update(zip(("host_q_lens", "host_k_lens", "host_q_starts", "host_q_pos_offsets"), per_row))

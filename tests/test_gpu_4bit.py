@@ -363,7 +363,7 @@ def test_rows_beyond_the_last_query_are_left(cuda, sea):
         q.data_ptr(), lib.i64_array(q.stride()), c.kv_cache.data_ptr(), c.kv_cache.stride(1), o.data_ptr(),
         lib.i64_array(o.stride()), l.data_ptr(), lib.i64_array(l.stride()), m["block_table"].data_ptr(),
         m["block_table_row_stride"], m["q_lens"].data_ptr(), m["k_lens"].data_ptr(), m["q_starts"].data_ptr(),
-        m["q_pos_offsets"].data_ptr(), 2, q.shape[0], 3, 50, 4, 2, 64, 16, c.num_blocks, step.scale, 1, 2, None, 0,
+        m["q_pos_offsets"].data_ptr(), 2, q.shape[0], 4, 3, 50, 4, 2, 64, 16, c.num_blocks, step.scale, 1, 2, None, 0,
         lib.stream_handle(cuda))
     lib.check(status, "kvhot_paged_attention_4bit")
     assert (o[4:] == 7).all() and (l[4:] == 7).all()

@@ -12,8 +12,15 @@ from test_gpu_4bit import BF16, FP16, FP32, Step, announce, f64
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True)
+def small_prompts(monkeypatch):
+    """Rows of these tests' sizes as prompts."""
+    monkeypatch.setattr(sea_module("kv_cache_4bit"), "PROMPT_FLOPS", 0)
+
+
 ROWS = [(1, 300, 299), (150, 400, 250), (3, 77, 74), (131, 131, 0), (1, 16, 15), (0, 9, 9), (200, 217, 17)]
-SHAPES = [(8, 2, 128, BF16), (8, 2, 64, FP16), (8, 2, 96, BF16), (4, 1, 256, FP16), (8, 2, 128, FP32), (8, 2, 64, FP32),
+SHAPES = [(8, 2, 128, BF16), (8, 2, 64, FP16), (8, 2, 96, BF16), (4, 1, 256, FP16), (16, 4, 128, FP16), (4, 1, 64, BF16),
           (12, 2, 64, BF16)]
 
 
@@ -96,8 +103,11 @@ def test_streams_and_captures(cuda, sea):
             step.check(*out)
 
 
-def test_short_rows_and_host_lengths_alone_decide(cuda, sea):
+def test_what_decides(cuda, sea, monkeypatch):
     kv4 = sea_module("kv_cache_4bit")
+    step = Step(sea, cuda, ROWS, 8, 2, 64, FP32)
+    step.check(*step.call(sea))
+    assert not taken(step)
     step = Step(sea, cuda, [(1, 300, 299), (20, 40, 20)], 8, 2, 64, BF16)
     step.check(*step.call(sea))
     assert not taken(step)
@@ -111,3 +121,13 @@ def test_short_rows_and_host_lengths_alone_decide(cuda, sea):
     assert not taken(step)
     step.check(o2, l2)
     assert np.abs(f64(o) - f64(o2)).max() < 0.05
+    monkeypatch.undo()
+    for n in (False, True):  # operations of all prompts below and at the bound
+        step = Step(sea, cuda, [(64, 1024 + 128, 1024 + 64)] * 8, 64, 8, 128, BF16)
+        monkeypatch.setattr(kv4, "PROMPT_FLOPS", 8 * 4 * 64 * 128 * 64 * 1120 * (2 if not n else 1))
+        announce("prompts' operations", n)
+        step.check(*step.call(sea))
+        assert taken(step) == n
+        native = sea_module("_lib").native().attention4(step.q, step.cache.blocks(0), step.meta, 64, 8, step.scale, True,
+                                                         sea_module("paged_attention_kernel")._WORKSPACES, kv4.PROMPT_PAIRS)
+        assert (native is not None) == (not n)

@@ -59,7 +59,8 @@ def test_calls_without_work_are_taken(lib):
     assert lib.kvhot_reshape_and_cache_4bit(*append_args(blocks=0, cache=None)) == 0
     assert lib.kvhot_read_cache_4bit(P, 4 * 17 * 128, None, 1, 0, 4, 128, 16, 10, None, None, 0, 2, None) == 0
     assert lib.kvhot_paged_attention_4bit(*attention_args(rows=0)) == 0
-    assert lib.kvhot_paged_attention_4bit(*attention_args(total=0)) == 0
+    assert lib.kvhot_paged_attention_4bit(*attention_args(total=0, sum_q=0)) == 0
+    assert lib.kvhot_paged_attention_4bit(*attention_args(sum_q=0)) == 0
     assert lib.kvhot_norm_rope(*rope_args(tokens=0)) == 0
 
 
@@ -75,7 +76,7 @@ def test_read_refusals(lib, kw, code):
 
 def attention_args(**kw):
     a = dict(q=P, qs=strides(1024, 128, 1), cache=P, block=4 * 17 * 128, out=P, os=strides(1024, 128, 1), lse=P,
-             ls=strides(8, 1), bt=P, bt_stride=40, q_lens=P, k_lens=P, q_starts=P, offs=P, rows=3, total=3, max_q=1,
+             ls=strides(8, 1), bt=P, bt_stride=40, q_lens=P, k_lens=P, q_starts=P, offs=P, rows=3, total=3, sum_q=3, max_q=1,
              max_k=600, hq=8, hkv=4, d=128, bs=16, blocks=10, scale=0.1, flags=1, dtype=2, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return list(a.values())
@@ -86,7 +87,7 @@ def attention_args(**kw):
     (dict(ls=None), EINVAL), (dict(qs=strides(1024, 1, 8)), EINVAL), (dict(hq=7), EINVAL), (dict(flags=2), EINVAL),
     (dict(flags=9), EINVAL), (dict(d=112), EUNSUPPORTED), (dict(bs=20), EUNSUPPORTED), (dict(dtype=3), EINVAL),
     (dict(blocks=0), EINVAL), (dict(max_k=1 << 33), EUNSUPPORTED), (dict(cache=P + 1), EINVAL), (dict(bt_stride=-1), EINVAL),
-    (dict(max_k=100000), EWORKSPACE), (dict(max_k=100000, ws=P, ws_bytes=64), EWORKSPACE), (dict(rows=-1), EINVAL),
+    (dict(max_k=100000), EWORKSPACE), (dict(sum_q=4), EINVAL), (dict(sum_q=-1), EINVAL), (dict(max_k=100000, ws=P, ws_bytes=64), EWORKSPACE), (dict(rows=-1), EINVAL),
 ])
 def test_attention_refusals(lib, kw, code):
     assert lib.kvhot_paged_attention_4bit(*attention_args(**kw)) == code
