@@ -487,7 +487,7 @@ __device__ inline void load_queries(const Attn4Args& a, const Block4& b, int lan
   for (int m = 0; m < MT; ++m) {
     const int at = 16 * m + n, mr = b.first + at;
     const bool there = at < b.rows;
-    const int tok = b.q0 + mr / a.group;
+    const int64_t tok = static_cast<int64_t>(b.q0) + mr / a.group;
     lim[m] = there ? sees(a, b, mr) : b.limit;
     const bool ok = there && tok >= 0 && tok < a.total_query;
     const typename IO::storage* src = static_cast<const typename IO::storage*>(a.q) +
@@ -544,7 +544,8 @@ __device__ inline void finish(const Attn4Args& a, const Block4& b, bool whole, i
     const float inv = sum == 0 ? 0.0f : 1.0f / sum;  // no key seen: 0
     const float lse2 = sum == 0 ? -INFINITY : st.ref[m] + F32::log2(sum);
     if (whole) {
-      const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
+      const int64_t tok = static_cast<int64_t>(b.q0) + mr / a.group;
+      const int hd = b.head * a.group + mr % a.group;
       if (tok < 0 || tok >= a.total_query) continue;
       typename IO::storage* o = static_cast<typename IO::storage*>(a.out) + tok * a.o_st + hd * a.o_sh;
 #pragma unroll
@@ -929,7 +930,8 @@ merge_4bit_kernel(Attn4Args a) {
   const int steps = (b.limit + kStep - 1) / kStep;
   const int parts = (steps + a.part_steps - 1) / a.part_steps;
   const int mr = b.first + m;
-  const int tok = b.q0 + mr / a.group, hd = b.head * a.group + mr % a.group;
+  const int64_t tok = static_cast<int64_t>(b.q0) + mr / a.group;
+  const int hd = b.head * a.group + mr % a.group;
   if (parts <= 1 || tok < 0 || tok >= a.total_query) return;
   const int64_t w0 = u * a.parts * a.hkv + head;
   float ref = -INFINITY, sum = 0, x[PER] = {};
@@ -1011,7 +1013,7 @@ spread_nan_4bit_kernel(Nan4Args n, int d) {
   if (any == INT32_MAX) return;
   const int n_q = imin(a.q_lens[r], a.max_q);
   for (int64_t i = threadIdx.x; i < static_cast<int64_t>(n_q) * a.group; i += 256) {
-    const int64_t tok = a.q_starts[r] + i / a.group;
+    const int64_t tok = static_cast<int64_t>(a.q_starts[r]) + i / a.group;
     const int h = head * a.group + static_cast<int>(i % a.group);
     const int64_t last = a.causal ? static_cast<int64_t>(a.q_offs[r]) + i / a.group : k_len - 1;
     if (tok < 0 || tok >= a.total_query) continue;

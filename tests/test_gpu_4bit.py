@@ -290,6 +290,52 @@ def test_extreme_scores(cuda, sea):
         step.check(o, l, q=q)
 
 
+def test_other_scales(cuda, sea):
+    """Negative (the largest scores are the smallest products) and zero (every key the same)."""
+    step = Step(sea, cuda, [(1, 400, 399), (6, 70, 64), (40, 40, 0)], 4, 2, 64, FP16)
+    for scale in (-0.3, 0.0):
+        step.scale = scale
+        announce("scale", scale)
+        o, l = step.call(sea)
+        step.scale = scale
+        want, lse, bound = step.expected(True)
+        assert (np.abs(f64(o) - want) <= 2.0 ** -9 * bound + 1e-6).all()
+        assert (np.abs(f64(l) - lse) <= 1e-4).all()
+
+
+def test_without_lse(cuda, sea):
+    step = Step(sea, cuda, [(1, 3000, 2999), (3, 70, 67)], 4, 2, 64, BF16)
+    lib = sea_module("_lib")
+    want, _ = step.call(sea)
+    m, c, q = step.meta, step.cache, step.q
+    o = torch.zeros_like(q)
+    need = lib.load().kvhot_paged_attention_4bit_workspace_bytes(2, 4, 3, 3000, 4, 2, 64, 2)
+    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=cuda)
+    announce("no lse")
+    lib.check(lib.load().kvhot_paged_attention_4bit(
+        q.data_ptr(), lib.i64_array(q.stride()), c.kv_cache.data_ptr(), c.kv_cache.stride(1), o.data_ptr(),
+        lib.i64_array(o.stride()), None, None, m["block_table"].data_ptr(), m["block_table_row_stride"], m["q_lens"].data_ptr(),
+        m["k_lens"].data_ptr(), m["q_starts"].data_ptr(), m["q_pos_offsets"].data_ptr(), 2, 4, 4, 3, 3000, 4, 2, 64, 16,
+        c.num_blocks, step.scale, 1, 2, ws.data_ptr(), need, lib.stream_handle(cuda)), "kvhot_paged_attention_4bit")
+    assert need > 0 and torch.equal(o, want)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, BF16), (64, 8, 64, FP16)])
+def test_many_rows_of_several_blocks(cuda, sea, hq, hkv, d, dtype):
+    """More rows than a wave, some without queries, of one to many query blocks:
+    the list of blocks on the device, one and two tiles a block."""
+    rng = np.random.default_rng(1)
+    for n, most in ((70, 3), (150, 12)):
+        rows = []
+        for i in range(n):
+            q = int(rng.integers(0, most)) if i % 5 else 0
+            k = int(rng.integers(max(q, 1), 90))
+            rows.append((q, k, k - q))
+        step = Step(sea, cuda, rows, hq, hkv, d, dtype)
+        announce("many rows", n, most, hq, hkv, d, dtype)
+        step.check(*step.call(sea))
+
+
 def test_pool_beyond_32_bits(cuda, sea):
     """Blocks whose bytes lie past 2^32 (17408 bytes a block)."""
     n = 300000
