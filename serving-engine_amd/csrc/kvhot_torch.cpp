@@ -20,6 +20,7 @@
 // all of these but the last two.
 #include <Python.h>
 
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
@@ -412,6 +413,7 @@ PyObject* py_read4(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return nullptr;
     const at::ScalarType type = dtype == KVHOT_F32 ? at::kFloat : dtype == KVHOT_F16 ? at::kHalf : at::kBFloat16;
     const auto options = p.pool.options().dtype(type);
+    const at::AutoDispatchBelowADInplaceOrView plain;  // (no gradients here: new tensors and views of them)
     const Tensor key = at::empty({slots.size(0), p.heads(), p.dim}, options), value = at::empty(key.sizes(), options);
     void* stream = c10::hip::getCurrentHIPStream(p.pool.get_device()).stream();
     const int status = without_gil([&] {
@@ -466,6 +468,7 @@ PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t need = g_workspace_bytes4(rows, q.size(0), max_q, max_k, hq, hkv, q.size(2), dt);
     void* stream = c10::hip::getCurrentHIPStream(d.index()).stream();
     if (need < 0 || (need > 0 && !stream_workspace(a[7], d, stream, need, ws))) return nullptr;
+    const at::AutoDispatchBelowADInplaceOrView plain;
     const Tensor o = at::empty_like(q, q.options().requires_grad(false)), l = lse_of(q);
     const int64_t qs[3] = {q.stride(0), q.stride(1), q.stride(2)}, os[3] = {o.stride(0), o.stride(1), o.stride(2)};
     const int64_t ls[2] = {l.stride(0), l.stride(1)};
@@ -507,6 +510,7 @@ PyObject* py_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
       wdt = dtype_code(w[i]);
     }
     const auto options = q.options().requires_grad(false);
+    const at::AutoDispatchBelowADInplaceOrView plain;
     const Tensor oq = at::empty(q.sizes(), options), ok = at::empty(k.sizes(), options);
     const Tensor* t[4] = {&q, &k, &oq, &ok};
     int64_t st[4][3];
@@ -543,6 +547,7 @@ PyObject* py_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !on_current_device(bt))
       return nullptr;
     const int64_t r = bt.size(0), mb = bt.size(1);
+    const at::AutoDispatchBelowADInplaceOrView plain;
     const Tensor ints = at::empty({2 * r + 1}, bt.options()), longs = at::empty({2 * total}, bt.options().dtype(at::kLong));
     int32_t* const i = static_cast<int32_t*>(ints.data_ptr());
     int64_t* const l = static_cast<int64_t*>(longs.data_ptr());
