@@ -342,6 +342,7 @@ def prepare(case, seed):
     c = {**_DEFAULTS, **case}
     s = _State()
     s.case = c
+    s.sea = _sea() if own else None
     if c["kind"] == "rope":
         s.q, s.k, s.wq, s.wk, s.positions, s.table = _rope_inputs(c, seed)
         return s
@@ -369,7 +370,7 @@ def prepare(case, seed):
         s.tables = [torch.tensor(t, device="cuda") for t in tables]
         s.scale = 1.0 / math.sqrt(c["d"])
     if own:
-        sea = _sea()
+        sea = s.sea
         s.cache = sea._PagedKVCache4Bit(s.pool, c["d"], dtype=DTYPES[c["dtype"]])
         if c["kind"] == "attention":
             s.meta = sea.step_inputs(_scheduled(sea, c, rows, tables), "cuda", s.cache)[0]
@@ -467,7 +468,7 @@ def run(state):
     s, c = state, state.case
     kind = c["kind"]
     if own:
-        sea = _sea()
+        sea = s.sea
         if kind == "rope":
             return sea.norm_rope(s.q, s.k, s.positions, s.table, s.wq, s.wk, eps=EPS, interleaved=c["interleaved"])
         if kind == "update":
