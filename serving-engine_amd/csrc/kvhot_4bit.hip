@@ -120,7 +120,8 @@ __device__ inline uint32_t quantise8(const float (&x)[8], uint32_t byte) {
 // A wave has 16 tokens of one head of K or V, GW groups of 32 elements in turn: lane
 // l has elements 8 (l / 16) on of token l % 16.  The 16 tokens of a prompt then lie
 // in the same lines of V, whose bytes of one pair are 16 tokens apart: with a
-// token's row in neighbouring lanes instead, 4152 tokens took 21 us.
+// token's row in neighbouring lanes instead, 4152 tokens of 8 heads took 21 us, so
+// 12.9 (22 MB, bound by its loads and 4-byte and 1-byte stores).
 struct Unit4 {
   int64_t t;  // the lane's token
   int32_t head, group;
@@ -217,9 +218,9 @@ __device__ inline void put(V x, void* p) {
 
 // A wave reads 16 slots of one head, K or V.  It writes whole rows, D / 8 lanes a
 // row, past the caches; K's codes are read in that order too.  V's are read as the
-// append writes them, tokens side by side, and change lanes in LDS: with 64-byte
-// pieces of 16 rows in a store instead, 90k tokens (480 MB in all) took 192 us
-// from HBM.
+// append writes them, tokens side by side, and change lanes in LDS.  Bound by HBM:
+// 90k tokens of 8 heads of 128 (480 MB in all) 119 us; with 64-byte pieces of 16
+// rows in a store instead 192, with ordinary stores 165 even from the caches.
 // BLOCKS: into kv-interleaved blocks of 16 tokens at `key` instead, NaN as 0, and
 // stored where the next kernel finds them.
 template <class T, typename SlotT, int D, bool BLOCKS>
@@ -787,46 +788,66 @@ __device__ inline void park(const State4<D, MT>& a, float* lds, int lane) {
 template <int D, int MT>
 constexpr int parked() { return MT * (D / 16 * 4 + 3) * kWave; }
 
-// The query block `flat` of all rows: of each 64 rows the one with the most keys
-// first, and its last block first (causal blocks' work grows along a row), so that
-// the longest start first.  (A grid of rows times the longest row's blocks would
-// launch work-groups for blocks that are not there, at 8 ns each.)
+// The sum of x over the wave's lanes up to this one.
+__device__ inline int64_t lanes_sum(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(x, o, kWave);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// The query block `flat` of all rows, the longest first: of up to 64 rows the one
+// with the most keys, and its last block (causal blocks' work grows along a row).
+// Of more rows each lane first sums a run of them, and the run that holds the block
+// is looked through in order (1000 rows of 2-9 queries: 64 rows after 64 instead,
+// sorted, 440 us).  (A grid of rows times the longest row's blocks would launch
+// work-groups for blocks that are not there, at 8 ns each.)
 template <int ROWS>
 __device__ inline bool flat_block(const Attn4Args& a, int64_t flat, int& row, int& qb) {
   const int lane = threadIdx.x & 63;
-  for (int r0 = 0; r0 < a.num_rows; r0 += 64) {
+  const auto blocks = [&](int r, int end) {
+    const int64_t n = r < end ? static_cast<int64_t>(imin(a.q_lens[r], a.max_q)) * a.group : 0;
+    return n > 0 ? (n + ROWS - 1) / ROWS : 0;
+  };
+  int first = 0, end = a.num_rows;
+  const bool many = a.num_rows > 64;
+  if (many) {
+    const int per = (a.num_rows + 63) / 64;
     int64_t mine = 0;
-    int keys = -1;
-    if (r0 + lane < a.num_rows) {
-      const int64_t n = static_cast<int64_t>(imin(a.q_lens[r0 + lane], a.max_q)) * a.group;
-      if (n > 0) {
-        mine = (n + ROWS - 1) / ROWS;
-        keys = a.k_lens[r0 + lane];
+    for (int j = 0; j < per; ++j) mine += blocks(lane * per + j, end);
+    const int64_t ends = lanes_sum(mine);
+    const uint64_t after = __ballot(ends > flat);
+    if (!after) return false;
+    const int at = __builtin_ctzll(after);
+    flat -= __shfl(ends - mine, at, kWave);
+    first = __builtin_amdgcn_readfirstlane(at * per);
+    end = imin(end, first + per);
+  }
+  for (; first < end; first += 64) {
+    int64_t mine = blocks(first + lane, end);
+    int from = lane;
+    if (!many) {
+      const int keys = mine > 0 ? a.k_lens[lane] : -1;
+      const uint64_t with = __ballot(mine > 0);
+      int rank = 0;  // rows that come before the lane's
+      for (uint64_t left = with; left; left &= left - 1) {
+        const int other = __builtin_ctzll(left), k = __builtin_amdgcn_readlane(keys, other);
+        rank += k > keys || (k == keys && other < lane) ? 1 : 0;
       }
+      // (lanes without blocks go behind the others, in their order)
+      if (mine == 0) rank = __popcll(with) + __popcll(~with & ((uint64_t{1} << lane) - 1));
+      from = __builtin_amdgcn_ds_permute(rank * 4, lane);  // the row of rank `lane`
+      mine = __shfl(mine, from, kWave);
     }
-    int rank = 0;  // rows that come before the lane's
-    for (uint64_t left = __ballot(mine > 0); left; left &= left - 1) {
-      const int other = __builtin_ctzll(left), k = __builtin_amdgcn_readlane(keys, other);
-      rank += k > keys || (k == keys && other < lane) ? 1 : 0;
-    }
-    // (lanes without blocks go behind the others, in their order)
-    const uint64_t with = __ballot(mine > 0);
-    if (mine == 0) rank = __popcll(with) + __popcll(~with & ((uint64_t{1} << lane) - 1));
-    const int from = __builtin_amdgcn_ds_permute(rank * 4, lane);  // the row of rank `lane`
-    mine = __shfl(mine, from, kWave);
-    int64_t ends = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t x = __shfl_up(ends, o, kWave);
-      if (lane >= o) ends += x;
-    }
+    const int64_t ends = lanes_sum(mine);
     const uint64_t after = __ballot(ends > flat);
     if (after) {
       const int at = __builtin_ctzll(after);
-      row = r0 + __shfl(from, at, kWave);
-      qb = static_cast<int>(__shfl(ends, at, kWave) - 1 - flat);
-      row = __builtin_amdgcn_readfirstlane(row);
-      qb = __builtin_amdgcn_readfirstlane(qb);
+      row = __builtin_amdgcn_readfirstlane(first + __shfl(from, at, kWave));
+      qb = __builtin_amdgcn_readfirstlane(static_cast<int>(__shfl(ends, at, kWave) - 1 - flat));
       return true;
     }
     flat -= __shfl(ends, 63, kWave);
@@ -846,6 +867,17 @@ __device__ inline bool grid_block(const Attn4Args& a, int64_t u, int& row, int& 
 // Waves a SIMD that the registers of an instantiation are for.
 constexpr int waves_per_simd(int np, int d, int mt) { return np == 3 ? (d == 256 ? 1 : 2) : d == 256 || mt == 2 ? 2 : 3; }
 
+// Attention over the cache: O^T = V^T P^T and S^T = K Q^T on the matrix cores, from
+// records that a wave loads straight into registers, with the running reference and
+// sum of a softmax.  Bound by HBM where rows are long (16 rows of 32768 keys at
+// 32 / 8 heads of 128: 106-110 us, 5.3 TB/s of 570 MB), by latency where they are
+// short (7-8 us of 1001 keys: lengths, block ids, records, the waves' join).  A step
+// is 64 keys so that a lane's probabilities are a whole record's; its phases are
+// kept apart by scheduling barriers, without which the conversions of a step were
+// all hoisted and one wave filled a SIMD (174 us).  Probabilities of 16-bit queries
+// are rounded to the type for the product with V: half a step of each weight, as
+// the output's own rounding; those of fp32 queries, and the queries, are three bf16
+// values each, whose products with the codes are exact.
 template <class IO, class M, int NP, int D, int MT>
 __global__ void __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NP, D, MT))))
 attn_4bit_kernel(Attn4Args a) {
@@ -1340,7 +1372,7 @@ extern "C" int kvhot_paged_attention_4bit(
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: null pointer");
   if (q_strides[2] != 1 || out_strides[2] != 1)
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: head_dim must be the innermost, unit-stride dim");
-  if (bt_row_stride < 0 || num_rows > 0x7fffffff) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
+  if (bt_row_stride < 0 || num_rows > 0x3fffffff) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
   if (num_blocks == 0 && max_k_len > 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: keys but no blocks");
   const Split4 sp = split_4bit(num_rows, sum_q_lens, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads,
                                head_dim, dtype);

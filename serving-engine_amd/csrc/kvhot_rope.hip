@@ -157,9 +157,9 @@ static int launch_rope(const RopeArgs& a, hipStream_t s) {
 template <class T>
 static int launch_rope(const RopeArgs& a, hipStream_t s) {
   // Outputs that pass the 8 L2s' 32 MiB: two sets of heads a wave, stored past
-  // the caches (8192 tokens of 40 heads of 128, bf16, 168 MB: 35.0 us = 4.8 TB/s;
-  // one set and ordinary stores 41.2, two 37.5, five 39.8, five past the caches
-  // 36.2).  Below that what is stored is read soon, and one set gives more waves.
+  // the caches (8192 tokens of 40 heads of 128, bf16, 168 MB, inputs in the last
+  // cache: 35.0 us; one set and ordinary stores 41.2, two 37.5, five 39.8, five
+  // past the caches 36.2; inputs from HBM: 44, three sets 47).  Below that what is stored is read soon, and one set gives more waves.
   const int64_t bytes = a.tokens * (a.hq + a.hkv) * a.d * static_cast<int64_t>(sizeof(typename T::storage));
   if (bytes >= (int64_t{32} << 20)) {
     if (a.d <= 64) return launch_rope<T, 8, 2>(a, s);

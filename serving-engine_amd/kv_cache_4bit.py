@@ -188,7 +188,9 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     stride), bf16, fp16 or fp32; kv_blocks: [num_blocks, block_size / 16,
     num_kv_heads, 17 * head_dim], a layer of the pool
     (``_PagedKVCache4Bit.blocks``); metadata: the dict of
-    build_paged_batch_metadata or build_block_tables.  Returns (o, l) as
+    build_paged_batch_metadata or build_block_tables (where the former's host
+    copies hold long prompts, those are planned from them, block table included,
+    once a step).  Returns (o, l) as
     paged_flash_attention does, the same bits on every call.  A NaN in the
     cache reaches the queries that see it and no other; in fp16, cached values beyond
     its range (of a pool written from another dtype) are infinite.

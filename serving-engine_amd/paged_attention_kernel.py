@@ -417,7 +417,8 @@ def build_block_tables(block_table, prior_lens, q_lens, free_blocks, total_query
     [R, MB], the lengths [R].  total_query: length of the slot mapping and the
     positions, at least the sum of q_lens (the tokens beyond it get slot -1,
     which an append skips, and position 0).  max_q_len and max_k_len (the
-    table's MB * block_size by default) bound the rows' lengths.
+    table's MB * block_size by default) bound the rows' lengths: they size the
+    attention's grid, so a close bound of a wide table's rows is worth passing.
 
     Returns the metadata dict of paged_flash_attention (and of
     paged_flash_attention_4bit), without host copies, plus ``slot_mapping``,

@@ -325,11 +325,11 @@ def test_many_rows_of_several_blocks(cuda, sea, hq, hkv, d, dtype):
     """More rows than a wave, some without queries, of one to many query blocks:
     the list of blocks on the device, one and two tiles a block."""
     rng = np.random.default_rng(1)
-    for n, most in ((70, 3), (150, 12)):
+    for n, most in ((64, 30), (70, 3), (150, 12), (4200, 3)):
         rows = []
         for i in range(n):
             q = int(rng.integers(0, most)) if i % 5 else 0
-            k = int(rng.integers(max(q, 1), 90))
+            k = int(rng.integers(max(q, 1), 90 if n < 1000 else 12))
             rows.append((q, k, k - q))
         step = Step(sea, cuda, rows, hq, hkv, d, dtype)
         announce("many rows", n, most, hq, hkv, d, dtype)
