@@ -453,7 +453,7 @@ PyObject* py_attention4(PyObject*, PyObject* const* a, Py_ssize_t n) {
         !as_int(PyDict_GetItemWithError(meta, g_names.max_k_len), max_k))
       return nullptr;
     PyObject* host = PyDict_GetItemWithError(meta, g_names.host_q_lens);
-    if (host && host != Py_None && dt != KVHOT_F32 && max_q * (hq / hkv) >= prompt) {
+    if (host && host != Py_None && dt != KVHOT_F32 && hq / hkv <= 16 && max_q * (hq / hkv) >= prompt) {
       PyObject* plans = PyDict_GetItemWithError(meta, g_names.schedules);
       if (!plans || !PyDict_CheckExact(plans)) return nullptr;
       char name[16];

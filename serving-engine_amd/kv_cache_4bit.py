@@ -190,10 +190,10 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     (``_PagedKVCache4Bit.blocks``); metadata: the dict of
     build_paged_batch_metadata or build_block_tables (where the former's host
     copies hold long prompts, those are planned from them, block table included,
-    once a step).  Returns (o, l) as
-    paged_flash_attention does, the same bits on every call.  A NaN in the
-    cache reaches the queries that see it and no other; in fp16, cached values beyond
-    its range (of a pool written from another dtype) are infinite.
+    once a step).  Returns (o, l) as paged_flash_attention does, the same bits on
+    every call.  A NaN in the cache reaches the queries that see it and no other; in
+    fp16, cached values beyond its range (of a pool written from another dtype) are
+    infinite.
     """
     out = _lib.native().attention4(q, kv_blocks, metadata, num_q_heads, num_kv_heads, scale, bool(is_causal), _WORKSPACES,
                                    PROMPT_PAIRS)
@@ -278,8 +278,10 @@ class _Prompts:
 # 103 / 92, of 512 186 / 149; 300 queries on 5000 keys, 24 GFLOP, 54 / 58; 16 / 4
 # heads of 256: 82 / 82, 155 / 108, 81 / 66).  In fp32, where the 4-bit kernel
 # multiplies in three bf16 parts and the other on the fp32 matrix cores, never:
-# 8 rows of 256 queries at 8 / 2 heads of 64 38 / 127.
+# 8 rows of 256 queries at 8 / 2 heads of 64 38 / 127.  Nor with groups of more than
+# PROMPT_GROUP heads, which the other kernels attend without matrix cores.
 PROMPT_PAIRS = 512
+PROMPT_GROUP = 16
 PROMPT_FLOPS = 35e9
 # Bytes that a call's copies may take.
 PROMPT_BYTES = 8 << 30
@@ -289,7 +291,7 @@ def _prompts(metadata, device, hq, hkv, d, block_size, dtype):
     """The step's _Prompts, planned from the host copies of its lengths and kept in
     the metadata; None without host copies or prompts."""
     host_q, group = metadata.get("host_q_lens"), hq // hkv
-    if (host_q is None or dtype == torch.float32
+    if (host_q is None or dtype == torch.float32 or group > PROMPT_GROUP
             or _host_max(metadata, "max_q_len", "q_lens") * group < PROMPT_PAIRS):
         return None
     key = ("prompts4", hq, hkv, d, block_size, _lib.dtype_code(dtype), str(device))
@@ -300,12 +302,13 @@ def _prompts(metadata, device, hq, hkv, d, block_size, dtype):
         return None if hit is None else hit[1]
     if torch.cuda.is_current_stream_capturing():
         return None  # (as _schedule: a copy from here would be replayed)
-    host_k, host_off = metadata["host_k_lens"], metadata["host_q_pos_offsets"]
+    host_k, host_bt = metadata["host_k_lens"], metadata["host_block_table"]
     rows = np.flatnonzero((host_q.astype(np.int64) * group >= PROMPT_PAIRS) & (host_k > 0))
     q_lens, k_lens = host_q[rows].astype(np.float64), host_k[rows].astype(np.int64)
     flops = 4.0 * hq * d * float((q_lens * (k_lens - q_lens / 2)).sum())  # causal
     blocks = -(-k_lens // BLOCK_SIZE)
-    if flops < PROMPT_FLOPS or int(blocks.sum()) * BLOCK_SIZE * hkv * d * 4 > PROMPT_BYTES:
+    if (flops < PROMPT_FLOPS or int(blocks.sum()) * BLOCK_SIZE * hkv * d * 4 > PROMPT_BYTES
+            or not rows.size or k_lens.max() > host_bt.shape[1] * block_size):
         cache[key] = None
         return None
     n = len(rows)
@@ -318,7 +321,7 @@ def _prompts(metadata, device, hq, hkv, d, block_size, dtype):
         table[i, :blocks[i]] = np.arange(first, ends[i])
         j = np.arange(k_lens[i])
         slots[first:ends[i]].reshape(-1)[:k_lens[i]] = (
-            metadata["host_block_table"][row, j // block_size].astype(np.int64) * block_size + j % block_size)
+            host_bt[row, j // block_size].astype(np.int64) * block_size + j % block_size)
     short = host_q.copy()
     short[rows] = 0
     left = np.flatnonzero(short > 0)
@@ -350,8 +353,8 @@ def _prompts(metadata, device, hq, hkv, d, block_size, dtype):
 
 def _attend_prompts(q, kv_blocks, metadata, p, bt_stride, scale, is_causal, o, l):
     """The prompts' attention: their keys as dense copies, once for all their
-    queries, then the 16- and 32-bit pools' attention over those, then the NaN
-    that the copies left out."""
+    queries, then the 16-bit pools' attention over those, then the NaN that the
+    copies left out."""
     lib, device, dtype = _lib.load(), q.device, _lib.dtype_code(q.dtype)
     num_blocks, spb, hkv, rec = kv_blocks.shape
     total_query, hq, d = q.shape

@@ -105,7 +105,13 @@ def test_streams_and_captures(cuda, sea):
 
 def test_what_decides(cuda, sea, monkeypatch):
     kv4 = sea_module("kv_cache_4bit")
-    step = Step(sea, cuda, ROWS, 8, 2, 64, FP32)
+    for hq, dtype in ((8, FP32), (34, BF16)):  # (17 heads to a kv head)
+        step = Step(sea, cuda, ROWS, hq, 2, 64, dtype)
+        announce("no prompts", hq, dtype)
+        step.check(*step.call(sea))
+        assert not taken(step)
+    step = Step(sea, cuda, ROWS, 8, 2, 64, BF16)
+    step.meta["host_block_table"] = step.meta["host_block_table"][:, :3]  # shorter than the rows
     step.check(*step.call(sea))
     assert not taken(step)
     step = Step(sea, cuda, [(1, 300, 299), (20, 40, 20)], 8, 2, 64, BF16)
