@@ -333,7 +333,7 @@ struct Attn4Args {
 };
 
 constexpr int kStep = 64;   // keys a wave attends at a time: four records
-constexpr int kWaves4 = 4;  // waves of a work-group, which share out its steps
+constexpr int kWaves4 = 4;  // most waves of a work-group, which share out its steps
 
 // One query block of one row and kv head: 16 * MT (query, head) pairs, "m-rows",
 // in the order query by query, against the key steps [step0, step1).
@@ -882,8 +882,9 @@ template <class IO, class M, int NP, int D, int MT>
 __global__ void __launch_bounds__(64 * kWaves4) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NP, D, MT))))
 attn_4bit_kernel(Attn4Args a) {
   constexpr int NJ = D / 32, ROWS = 16 * MT;
-  __shared__ float lds[kWaves4 / 2 * parked<D, MT>()];
+  extern __shared__ float lds[];  // half of the waves' states
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = static_cast<int>(blockDim.x) >> 6;
   int64_t u = blockIdx.x;
   const int head = static_cast<int>(u % a.hkv);
   u /= a.hkv;
@@ -909,7 +910,7 @@ attn_4bit_kernel(Attn4Args a) {
     Where4 w = where(a, b, s, lane);
     load_keys<D>(a, b, w, lane, keys);
     load_values<D>(a, b, w, lane, values);
-    w = where(a, b, imin(s + kWaves4, step1 - 1), lane);
+    w = where(a, b, imin(s + waves, step1 - 1), lane);
     const auto step = [&](auto masked) {
       constexpr bool MASKED = decltype(masked)::value;
       f32x4 sc[MT][4];
@@ -922,22 +923,22 @@ attn_4bit_kernel(Attn4Args a) {
       __builtin_amdgcn_sched_barrier(0);
       weigh<M, NP, D, MT, MASKED>(values, p, lim, s * kStep, b.limit, lane, st);
       load_values<D>(a, b, w, lane, values);
-      w = where(a, b, imin(s + 2 * kWaves4, step1 - 1), lane);
-      s += kWaves4;
+      w = where(a, b, imin(s + 2 * waves, step1 - 1), lane);
+      s += waves;
     };
     const int full = imin(step1, b.least / kStep);  // steps that every m-row sees whole
     while (s < full) step(std::false_type());
     while (s < step1) step(std::true_type());
   }
-  // The waves' states, joined in LDS: 2 and 3 into 0 and 1, then 1 into 0.
-  if (wave >= 2) park<D, MT>(st, lds + (wave - 2) * parked<D, MT>(), lane);
-  __syncthreads();
-  if (wave < 2) join<D, MT>(st, lds + wave * parked<D, MT>(), lane);
-  __syncthreads();
-  if (wave == 1) park<D, MT>(st, lds, lane);
-  __syncthreads();
+  // The waves' states, joined in LDS: the upper half into the lower until one is
+  // left (of 4 waves 2 and 3 into 0 and 1, then 1 into 0).
+  for (int half = waves / 2; half > 0; half >>= 1) {
+    if (wave >= half && wave < 2 * half) park<D, MT>(st, lds + (wave - half) * parked<D, MT>(), lane);
+    __syncthreads();
+    if (wave < half) join<D, MT>(st, lds + wave * parked<D, MT>(), lane);
+    __syncthreads();
+  }
   if (wave != 0) return;
-  join<D, MT>(st, lds, lane);
 
   const int64_t w = (u * a.parts + part) * a.hkv + head;
   finish<IO, D, MT>(a, b, steps <= a.part_steps, w * ROWS, lane, st);
@@ -1059,10 +1060,11 @@ spread_nan_4bit_kernel(Nan4Args n, int d) {
 
 constexpr int64_t kWholeSteps = 128;
 
-// Split of a call: tiles of 16 m-rows of a query block, blocks (of all rows), parts,
-// key steps of a part, and the workspace: partials, then their logarithms.
+// Split of a call: tiles of 16 m-rows of a query block, blocks (of all rows), waves
+// of a work-group, parts, key steps of a part, and the workspace: partials, then
+// their logarithms.
 struct Split4 {
-  int32_t mt, flat, parts, part_steps;
+  int32_t mt, flat, waves, parts, part_steps;
   int64_t blocks, ws_bytes;
 };
 
@@ -1088,6 +1090,12 @@ static Split4 split_4bit(int64_t rows, int64_t total, int64_t max_q, int64_t max
   // (24 rows of up to 6000 keys: 20.9 us, 24.9 when cut for three).
   const int64_t n = std::max<int64_t>(s.blocks * hkv, 1);
   const int64_t parts = n >= 512 ? 1 : (1024 + n - 1) / n;
+  // Where blocks of up to 16 steps fill the CUs' waves without it, a block is one
+  // wave's or two's: a start and a join then serve more steps (us with 4 waves, 2
+  // and 1; 256 rows of up to 128 keys 23.1 / 16.6 / 12.8, of up to 1024 49.4 / 46.7 /
+  // 44.8, of up to 2048 74 / 80 / 78; 128 rows of up to 1024 30.9 / 26.7 / 30.4, of
+  // up to 4096 80 / 80 / 99; 1000 rows of 2-9 queries 316 / 194 / 136).
+  s.waves = steps > 16 || n < 768 ? kWaves4 : n < 1536 ? 2 : 1;
   // A part has a step a wave at least; rows of two steps a wave stay whole (a row
   // of 1001 keys in parts of two 11.1 us, of one 10.2, a merge of 2.5 in both).
   const int64_t few = steps <= 2 * kWaves4 ? 2 * kWaves4 : kWaves4;
@@ -1247,8 +1255,9 @@ int launch_4bit(const Split4& sp, const Attn4Args& a, hipStream_t s) {
   const int64_t blocks = sp.blocks * a.hkv;
   if (blocks * std::max<int64_t>(sp.parts, 4 * MT) > 0x7fffffff)
     return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
+  const size_t lds = static_cast<size_t>(sp.waves / 2) * parked<D, MT>() * sizeof(float);
   hipLaunchKernelGGL((attn_4bit_kernel<IO, M, NP, D, MT>), dim3(static_cast<uint32_t>(blocks * sp.parts)),
-                     dim3(64 * kWaves4), 0, s, a);
+                     dim3(64 * static_cast<uint32_t>(sp.waves)), lds, s, a);
   if (int e = launch_status("paged_attention_4bit")) return e;
   if (sp.parts == 1) return 0;
   hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks * (4 * MT))), dim3(256), 0, s,

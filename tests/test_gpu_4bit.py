@@ -336,6 +336,21 @@ def test_many_rows_of_several_blocks(cuda, sea, hq, hkv, d, dtype):
         step.check(*step.call(sea))
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(16, 8, 128, BF16), (8, 8, 64, FP32)])
+@pytest.mark.parametrize("n,most", [(95, 200), (96, 1024), (96, 1025), (191, 130), (192, 130)])
+def test_many_short_rows(cuda, sea, hq, hkv, d, dtype, n, most):
+    """Single tokens' rows around the numbers and lengths where a work-group has one,
+    two and four waves; rows without keys and one that reaches the length."""
+    rng = np.random.default_rng(2)
+    lens = [most, 0, 1, 65] + [int(x) for x in rng.integers(0, most + 1, n - 4)]
+    step = Step(sea, cuda, [(1, k, k - 1) for k in lens], hq, hkv, d, dtype)
+    announce("many short rows", n, most, hq, hkv, d, dtype)
+    o, l = step.call(sea)
+    step.check(o, l)
+    o2, l2 = step.call(sea)
+    assert torch.equal(o, o2) and torch.equal(l, l2)
+
+
 def test_pool_beyond_32_bits(cuda, sea):
     """Blocks whose bytes lie past 2^32 (17408 bytes a block)."""
     n = 300000
