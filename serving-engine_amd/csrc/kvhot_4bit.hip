@@ -1232,7 +1232,7 @@ static int check_attention(int64_t rows, int64_t total, int64_t max_q, int64_t m
   if (hq % hkv != 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: num_q_heads must be a multiple of num_kv_heads");
   if (dtype_size(dtype) == 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad dtype");
   if (!head_dim_4bit(d)) return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: head_dim must be 64, 96, 128 or 256");
-  if (max_k > 0x7fffff00 || max_q > 0x7fffff00 || hq > (1 << 16) || max_q * (hq / hkv) > 0x7fffff00)
+  if (max_k > 0x7fffff00 || max_q > 0x7fffff00 || rows > 0x3fffffff || total > 0x7fffffff || hq > (1 << 16) || max_q * (hq / hkv) > 0x7fffff00)
     return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: sizes beyond the kernels' range");
   return 0;
 }
@@ -1381,7 +1381,7 @@ extern "C" int kvhot_paged_attention_4bit(
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: null pointer");
   if (q_strides[2] != 1 || out_strides[2] != 1)
     return set_error(KVHOT_EINVAL, "paged_attention_4bit: head_dim must be the innermost, unit-stride dim");
-  if (bt_row_stride < 0 || num_rows > 0x3fffffff) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
+  if (bt_row_stride < 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: bad sizes");
   if (num_blocks == 0 && max_k_len > 0) return set_error(KVHOT_EINVAL, "paged_attention_4bit: keys but no blocks");
   const Split4 sp = split_4bit(num_rows, sum_q_lens, max_q_len, max_k_len, num_q_heads / num_kv_heads, num_kv_heads,
                                head_dim, dtype);

@@ -191,9 +191,10 @@ def paged_flash_attention_4bit(q, kv_blocks, metadata, num_q_heads, num_kv_heads
     build_paged_batch_metadata or build_block_tables (where the former's host
     copies hold long prompts, those are planned from them, block table included,
     once a step).  Returns (o, l) as paged_flash_attention does, the same bits on
-    every call.  A NaN in the cache reaches the queries that see it and no other; in
-    fp16, cached values beyond its range (of a pool written from another dtype) are
-    infinite.
+    every call.  A NaN in the cache reaches the queries that see it and no other.
+    A pool written in another dtype may hold values beyond fp16's range; with fp16
+    queries those are infinite, and an infinite value may also reach queries of a
+    long prompt that do not see it.
     """
     out = _lib.native().attention4(q, kv_blocks, metadata, num_q_heads, num_kv_heads, scale, bool(is_causal), _WORKSPACES,
                                    PROMPT_PAIRS)

@@ -231,6 +231,35 @@ def test_larger_blocks(cuda, sea, bs):
     step.check(*step.call(sea))
 
 
+@pytest.mark.parametrize("rows", ["decode", "drafts", "prompts"])
+def test_blocks_of_a_wider_pool(cuda, sea, rows):
+    """Blocks with other bytes between them, layers too."""
+    step = Step(sea, cuda, ROWS[rows], 8, 2, 128, BF16, bs=32)
+    o, l = step.call(sea)
+    pool = step.cache.kv_cache
+    wide = torch.full((2, 2 * pool.shape[1], *pool.shape[2:]), 255, dtype=torch.uint8, device=cuda)  # NaN
+    wide[1, ::2] = pool[0]
+    step.cache = sea._PagedKVCache4Bit(wide[:, ::2], 128, BF16)
+    announce("blocks of a wider pool", rows)
+    o2, l2 = sea.paged_flash_attention_4bit(step.q, step.cache.blocks(1), step.meta, 8, 2, step.scale)
+    assert torch.equal(o, o2) and torch.equal(l, l2)
+
+
+@pytest.mark.parametrize("rows", ["decode", "drafts"])
+def test_pages_outside_the_pool_stay_inside(cuda, sea, rows):
+    """Block ids that no block has, in one row: the others' results are as they were."""
+    step = Step(sea, cuda, ROWS[rows], 8, 2, 64, FP16)
+    o, l = step.call(sea)
+    bad = len(ROWS[rows]) - 2
+    lo, hi = int(step.starts[bad]), int(step.starts[bad + 1])
+    for page in (-1, step.cache.num_blocks, 2 ** 31 - 1, -2 ** 31):
+        step.meta["block_table"][bad] = page
+        announce("pages outside the pool", rows, page)
+        o2, l2 = step.call(sea)
+        for got, want in ((o2, o), (l2, l)):
+            assert torch.equal(got[:lo], want[:lo]) and torch.equal(got[hi:], want[hi:])
+
+
 @pytest.mark.parametrize("rows", [[(1, 20000, 19999)], [(3, 9001, 8998), (1, 33, 32)], [(300, 5000, 4700)],
                                   [(1, 4000 - 7 * i, 3999 - 7 * i) for i in range(40)] + [(200, 200, 0)]])
 @pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, BF16), (2, 2, 64, FP16), (4, 1, 256, FP32)])

@@ -210,3 +210,12 @@ def test_reference_quantiser():
     assert ref.quantise(np.array([7.0] + [0] * 31)[None], "bfloat16")[1][0, 0] == 127
     assert ref.quantise(np.array([7.0625] + [0] * 31)[None], "bfloat16")[1][0, 0] == 128
     assert ref.quantise(np.array([np.inf] + [0] * 31)[None], "bfloat16")[1][0, 0] == 255
+
+
+@pytest.mark.parametrize("kw", [dict(rows=1 << 30), dict(total=1 << 31), dict(total=1 << 62, sum_q=1 << 62), dict(max_q=1 << 31),
+                                dict(hq=1 << 17, hkv=1 << 17)])
+def test_attention_sizes_beyond_the_kernels(lib, kw):
+    assert lib.kvhot_paged_attention_4bit(*attention_args(**kw)) == EUNSUPPORTED
+    a = dict(rows=3, total=3, max_q=1, max_k=600, hq=8, hkv=4, d=128, dtype=2)
+    a.update({k: v for k, v in kw.items() if k in a})
+    assert lib.kvhot_paged_attention_4bit_workspace_bytes(*a.values()) == EUNSUPPORTED
