@@ -944,21 +944,23 @@ attn_4bit_kernel(Attn4Args a) {
   finish<IO, D, MT>(a, b, steps <= a.part_steps, w * ROWS, lane, st);
 }
 
-// Joins the parts of the query blocks that were cut: one wave an m-row, eight
-// parts on their way at a time.
-template <class IO, int D, int ROWS>
+// Joins the parts of the query blocks that were cut: WAVES (1 or 4) waves an m-row,
+// each with a run of its parts, eight on their way at a time.  Bound by those loads'
+// latency, 1.2 us for eight parts.
+template <class IO, int D, int ROWS, int WAVES>
 __global__ void __launch_bounds__(256)
 merge_4bit_kernel(Attn4Args a) {
-  constexpr int PER = (D + 63) / 64, AHEAD = 8;
+  constexpr int PER = (D + 63) / 64, AHEAD = 8, SETS = ROWS * WAVES / 4;  // work-groups of a block
+  __shared__ float lds[WAVES == 4 ? 3 * (PER + 2) * kWave : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t u = blockIdx.x;
-  const int quarter = static_cast<int>(u % (ROWS / 4));  // m-rows 4 * quarter + wave
-  u /= ROWS / 4;
+  const int set = static_cast<int>(u % SETS);
+  u /= SETS;
   const int head = static_cast<int>(u % a.hkv);
   u /= a.hkv;
   int row, qb;
   Block4 b;
-  const int m = quarter * 4 + wave;
+  const int m = WAVES == 4 ? set : set * 4 + wave;
   if (!grid_block<ROWS>(a, u, row, qb) || !block_of<ROWS>(a, row, head, qb, b) || m >= b.rows) return;
   const int steps = (b.limit + kStep - 1) / kStep;
   const int parts = (steps + a.part_steps - 1) / a.part_steps;
@@ -967,14 +969,16 @@ merge_4bit_kernel(Attn4Args a) {
   const int hd = b.head * a.group + mr % a.group;
   if (parts <= 1 || tok < 0 || tok >= a.total_query) return;
   const int64_t w0 = u * a.parts * a.hkv + head;
+  const int run = WAVES == 4 ? (parts + 3) / 4 : parts, begin = WAVES == 4 ? imin(wave * run, parts) : 0;
+  const int end = imin(begin + run, parts);
   float ref = -INFINITY, sum = 0, x[PER] = {};
-  for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+  for (int p0 = begin; p0 < end; p0 += AHEAD) {
     float l[AHEAD], y[AHEAD][PER];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int p = imin(p0 + k, parts - 1);
+      const int p = imin(p0 + k, end - 1);
       const int64_t w = (w0 + static_cast<int64_t>(p) * a.hkv) * ROWS + m;
-      l[k] = p0 + k < parts ? a.ws_lse[w] : -INFINITY;
+      l[k] = p0 + k < end ? a.ws_lse[w] : -INFINITY;
 #pragma unroll
       for (int i = 0; i < PER; ++i) y[k][i] = i * 64 + lane < D ? a.ws_o[w * D + i * 64 + lane] : 0.0f;
     }
@@ -989,11 +993,41 @@ merge_4bit_kernel(Attn4Args a) {
     for (int i = 0; i < PER; ++i) x[i] *= keep;
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      if (p0 + k >= parts) break;
+      if (p0 + k >= end) break;
       const float f = F32::exp2(l[k] - base);
       sum += f;
 #pragma unroll
       for (int i = 0; i < PER; ++i) x[i] += f * y[k][i];
+    }
+  }
+  if constexpr (WAVES == 4) {  // (the m-row, and so every return above, is the work-group's)
+    if (wave > 0) {
+      float* p = lds + (wave - 1) * (PER + 2) * kWave + lane;
+      p[0] = ref;
+      p[kWave] = sum;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) p[(2 + i) * kWave] = x[i];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float top = ref;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const float l = lds[k * (PER + 2) * kWave + lane];
+      top = l > top || l != l ? l : top;
+    }
+    const float base = top == -INFINITY ? 0.0f : top, keep = F32::exp2(ref - base);
+    ref = top;
+    sum *= keep;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] *= keep;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const float* p = lds + k * (PER + 2) * kWave + lane;
+      const float f = F32::exp2(p[0] - base);
+      sum += f * p[kWave];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] += f * p[(2 + i) * kWave];
     }
   }
   const float inv = sum == 0 ? 0.0f : 1.0f / sum;
@@ -1087,9 +1121,13 @@ static Split4 split_4bit(int64_t rows, int64_t total, int64_t max_q, int64_t max
   // kWholeSteps steps (64 rows of 128-2048 keys: 23.6 us, in two parts 25.7 and
   // a merge of 4.8); fewer are cut for four work-groups a CU, of which three
   // fit: rows are ragged, and the parts behind a short row's end are empty
-  // (24 rows of up to 6000 keys: 20.9 us, 24.9 when cut for three).
+  // (24 rows of up to 6000 keys: 24.2 us, 26.9 when cut for three).  Up to 128,
+  // rows of many parts, for those that fit (us cut for four and for three: a row of
+  // 32768 keys 17.9 / 15.2, 4 of 16384 26.0 / 22.1, 8 38.7 / 35.0, of 1000-16384
+  // 24.6 / 22.4, 16 of 8192 38.3 / 34.5; 4 of 1000-16384 16.8 / 17.8).
   const int64_t n = std::max<int64_t>(s.blocks * hkv, 1);
-  const int64_t parts = n >= 512 ? 1 : (1024 + n - 1) / n;
+  const int64_t fit = 256 * waves_per_simd(dtype == KVHOT_F32 ? 3 : 1, static_cast<int>(d), s.mt);
+  const int64_t parts = n >= 512 ? 1 : n > 128 ? (1024 + n - 1) / n : std::max<int64_t>(fit / n, 1);
   // Where blocks of up to 16 steps fill the CUs' waves without it, a block is one
   // wave's or two's: a start and a join then serve more steps (us with 4 waves, 2
   // and 1; 256 rows of up to 128 keys 23.1 / 16.6 / 12.8, of up to 1024 49.4 / 46.7 /
@@ -1253,15 +1291,22 @@ namespace {
 template <class IO, class M, int NP, int D, int MT>
 int launch_4bit(const Split4& sp, const Attn4Args& a, hipStream_t s) {
   const int64_t blocks = sp.blocks * a.hkv;
-  if (blocks * std::max<int64_t>(sp.parts, 4 * MT) > 0x7fffffff)
+  if (blocks * std::max<int64_t>(sp.parts, 16 * MT) > 0x7fffffff)
     return set_error(KVHOT_EUNSUPPORTED, "paged_attention_4bit: too many work-groups");
   const size_t lds = static_cast<size_t>(sp.waves / 2) * parked<D, MT>() * sizeof(float);
   hipLaunchKernelGGL((attn_4bit_kernel<IO, M, NP, D, MT>), dim3(static_cast<uint32_t>(blocks * sp.parts)),
                      dim3(64 * static_cast<uint32_t>(sp.waves)), lds, s, a);
   if (int e = launch_status("paged_attention_4bit")) return e;
   if (sp.parts == 1) return 0;
-  hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT>), dim3(static_cast<uint32_t>(blocks * (4 * MT))), dim3(256), 0, s,
-                     a);
+  // Parts of more than one trip are four waves' (us with one and four: 96 parts 15.4 /
+  // 5.6, 43 7.5 / 3.8, 24 6.6 / 4.2, 12 4.9 / 4.8; one trip, 6 parts of 192 blocks,
+  // 5.4 / 8.0: the work-groups are four times as many).
+  if (sp.parts > 8)
+    hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT, 4>), dim3(static_cast<uint32_t>(blocks * (16 * MT))), dim3(256), 0,
+                       s, a);
+  else
+    hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT, 1>), dim3(static_cast<uint32_t>(blocks * (4 * MT))), dim3(256), 0,
+                       s, a);
   return launch_status("paged_attention_4bit merge");
 }
 

@@ -272,6 +272,23 @@ def test_long_rows_cut_into_parts(cuda, sea, rows, hq, hkv, d, dtype):
     step.check(*step.call(sea))
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(6, 2, 96, BF16), (4, 1, 64, FP16), (2, 2, 256, BF16), (20, 1, 128, FP16), (2, 1, 96, FP32)])
+def test_long_rows_in_many_parts(cuda, sea, hq, hkv, d, dtype):
+    """One row and a few of many parts; some without queries, short or seen in part."""
+    for rows in ([(1, 33333, 33332)], [(2, 9000, 8990), (0, 7000, 7000), (1, 5, 4), (3, 20001, 19998)]):
+        step = Step(sea, cuda, rows, hq, hkv, d, dtype)
+        announce("many parts", rows, hq, hkv, d, dtype)
+        for causal in (True, False):
+            step.check(*step.call(sea, causal), causal)
+
+
+def test_long_prompts_of_two_tiles_in_parts(cuda, sea):
+    """A prompt of 1024 blocks of one tile on more keys than a block takes whole."""
+    step = Step(sea, cuda, [(512, 8500, 7988)], 32, 2, 64, FP16, device_only=True)
+    announce("two tiles in parts")
+    step.check(*step.call(sea))
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 def test_queries_of_any_strides(cuda, sea, dtype):
     step = Step(sea, cuda, ROWS["drafts"], 4, 2, 64, dtype)
