@@ -1298,8 +1298,8 @@ int launch_4bit(const Split4& sp, const Attn4Args& a, hipStream_t s) {
                      dim3(64 * static_cast<uint32_t>(sp.waves)), lds, s, a);
   if (int e = launch_status("paged_attention_4bit")) return e;
   if (sp.parts == 1) return 0;
-  // Parts of more than one trip are four waves' (us with one and four: 96 parts 15.4 /
-  // 5.6, 43 7.5 / 3.8, 24 6.6 / 4.2, 12 4.9 / 4.8; one trip, 6 parts of 192 blocks,
+  // Parts of more than one trip are four waves' (us with one and four: 86 parts 15.4 /
+  // 5.6, 32 7.5 / 3.8, 24 6.6 / 4.2, 12 4.9 / 4.8; one trip, 6 parts of 192 blocks,
   // 5.4 / 8.0: the work-groups are four times as many).
   if (sp.parts > 8)
     hipLaunchKernelGGL((merge_4bit_kernel<IO, D, 16 * MT, 4>), dim3(static_cast<uint32_t>(blocks * (16 * MT))), dim3(256), 0,
